@@ -1,0 +1,444 @@
+"""What the transformer-layer operators of ``pointcloudmatters_amd.policy`` are measured on: rotary positions over several axes,
+cross attention to an encoder's states of another length, and the gated feed-forward block, each beside its plain form.
+
+``run`` computes a case in elementary 32-bit operations (``own = False``) or with the framework's calls (``own = True``); ``exact``
+gives the same outputs from the definitions in 64 bits.
+
+Definitions
+-----------
+rotary   Pair j (of n_a) of axis a turns by  coords[..., a] * base ** (-j / n_a)  radians.  With R = 2 * sum(n_a) turned channels the
+         pairs are (i, i + R / 2), or (2 i, 2 i + 1) when interleaved; channels from R on pass through.
+cross    softmax(scale * q k^T) v per head over the keys that a row's sequence holds and the mask leaves; a row without a key is zero.
+         Query head h reads key head h // (H / Hkv).  Packed sides hold sequence i in rows [offset[i - 1], offset[i]).
+ffn      (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd.
+"""
+import math
+import random
+
+import torch
+
+own = False
+
+DEV = "cuda"
+TYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+# ---- the cases -----------------------------------------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # one token of a rollout, eight heads of 64: a launch and little else
+        dict(name="rotary-one-token", op="rotary", rows=1, heads=8, dim=64, sections="11,11,10", dtype="bf16", whole=False, far=0,
+             interleaved=False, train=False),
+        # the queries and keys of one encoder layer over eight clouds of 2048 tokens + 3, in metres / voxel size, forward and backward
+        dict(name="rotary-tokens-train", op="rotary", rows=8 * 2051, heads=16, dim=64, sections="11,11,10", dtype="bf16", whole=False,
+             far=0, interleaved=False, train=True),
+        # whole voxel indices far from the origin (a map, a long video), 32-bit values, a part of the head turned
+        dict(name="rotary-far-fp32", op="rotary", rows=65521, heads=16, dim=128, sections="16,20,20", dtype="fp32", whole=True,
+             far=1 << 20, interleaved=True, train=False),
+        # one query of one rollout against one cloud's tokens
+        dict(name="cross-one-query", op="cross", batch=1, queries=1, keys=2051, heads=8, kv_heads=8, dim=64, packed_q=False,
+             packed_kv=True, masked=False, train=False),
+        # the decoder's 100 action queries against eight ragged clouds of about 2000 tokens, forward and backward
+        dict(name="cross-decoder-train", op="cross", batch=8, queries=100, keys=2600, heads=8, kv_heads=8, dim=64, packed_q=False,
+             packed_kv=True, masked=False, train=True),
+        # padded token sets with padding in any place, shared key heads, wide heads, forward and backward
+        dict(name="cross-masked-train", op="cross", batch=4, queries=515, keys=1027, heads=16, kv_heads=4, dim=128, packed_q=False,
+             packed_kv=False, masked=True, train=True),
+        # many latent queries reading a large scene
+        dict(name="cross-scene", op="cross", batch=4, queries=2048, keys=16384, heads=8, kv_heads=8, dim=64, packed_q=True,
+             packed_kv=True, masked=False, train=False),
+        # 64 rollouts stepped together, one token each, against stored states with two key heads
+        dict(name="cross-step-batch", op="cross", batch=64, queries=1, keys=8192, heads=16, kv_heads=2, dim=128, packed_q=False,
+             packed_kv=True, masked=False, train=False),
+        # one token through the block; a hidden width of 8 / 3 of the model's, which is odd
+        dict(name="ffn-one-row", op="ffn", rows=1, width=512, hidden=1365, act="silu", bias=False, train=False),
+        # the decoder's rows of a training step at the same width
+        dict(name="ffn-decoder-train", op="ffn", rows=800, width=512, hidden=1365, act="silu", bias=True, train=True),
+        # the encoder's rows of a training step
+        dict(name="ffn-tokens-train", op="ffn", rows=8 * 2051, width=512, hidden=2048, act="gelu", bias=True, train=True),
+        # a wide model's forward pass
+        dict(name="ffn-wide", op="ffn", rows=8192, width=2048, hidden=5632, act="silu", bias=False, train=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["rotary", "cross", "cross", "ffn"])
+    if op == "rotary":
+        heads, dim = rng.choice([1, 2, 5, 8, 16, 32]), rng.choice([32, 64, 72, 96, 128])
+        axes = rng.choice([1, 2, 3, 4])
+        left, sections = dim // 2, []
+        for a in range(axes):
+            n = rng.randint(1, max(1, left // (axes - a)))
+            sections.append(n)
+            left -= n
+        whole = rng.random() < 0.5
+        return dict(op="rotary", rows=_log(rng, 1, 120e6 / (heads * dim)), heads=heads, dim=dim, sections=",".join(map(str, sections)),
+                    dtype=rng.choice(["bf16", "fp32"]), whole=whole, far=rng.choice([0, 1 << 20]) if whole else 0,
+                    interleaved=rng.random() < 0.5, train=rng.random() < 0.5)
+    if op == "cross":
+        heads, kv_heads = rng.choice([(8, 8), (4, 4), (8, 2), (16, 4), (6, 2), (5, 1), (16, 16)])
+        dim, train = rng.choice([32, 64, 64, 80, 128]), rng.random() < 0.5
+        batch, keys = _log(rng, 1, 32), _log(rng, 16 if train else 1, 16384)  # one key alone has no gradient to compare: its weight is 1
+        most = 1.2e11 / (4 * batch * heads * dim * keys * (3.5 if train else 1))
+        most = min(most, 1.0e9 / (batch * heads * keys), 1.0e8 / (batch * heads * dim), 2048)
+        packed = rng.random() < 0.5
+        return dict(op="cross", batch=batch, queries=_log(rng, 1, max(1, most)), keys=keys, heads=heads, kv_heads=kv_heads, dim=dim,
+                    packed_q=rng.random() < 0.5, packed_kv=packed, masked=not packed and rng.random() < 0.7, train=train)
+    train = rng.random() < 0.5
+    width, hidden = rng.choice([256, 384, 512, 768, 1024, 500]), _log(rng, 256, 4096)
+    most = 2.5e11 / (6 * width * hidden * (3 if train else 1))
+    return dict(op="ffn", rows=_log(rng, 1, min(32768, most)), width=width, hidden=hidden, act=rng.choice(["silu", "gelu", "relu"]),
+                bias=rng.random() < 0.5, train=train)
+
+
+# ---- the inputs ----------------------------------------------------------------------------------------------------------------
+
+def _normal(g, *shape, scale=1.0, dtype=torch.bfloat16):
+    return (torch.randn(*shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def _lengths(case, side):
+    """Rows of each sequence: all of them on a padded side, ragged between half and all of them on a packed one (the same for every
+    seed: other inputs of a case have its shapes); from three sequences on, the second of a packed side is empty."""
+    batch, most, packed = (case["batch"], case["queries"], case["packed_q"]) if side == "q" else (case["batch"], case["keys"], case["packed_kv"])
+    if not packed or most == 1:
+        return [most] * batch
+    rng = random.Random(batch * 1000003 + most)
+    lens = [rng.randint((most + 1) // 2, most) for _ in range(batch)]
+    if batch >= 3:
+        lens[1] = 0
+    return lens
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    st = dict(case=dict(case))
+    if case["op"] == "rotary":
+        t, h, d = case["rows"], case["heads"], case["dim"]
+        sections = tuple(int(s) for s in case["sections"].split(","))
+        dtype = TYPES[case["dtype"]]
+        st["sections"] = sections
+        st["x"] = _normal(g, t, h, d, dtype=dtype).requires_grad_(case["train"])
+        st["coords"] = _coords(g, t, len(sections), case)
+        if case["train"]:
+            st["dout"] = _normal(g, t, h, d, dtype=dtype)
+        return st
+    if case["op"] == "cross":
+        b, lq, lk, h, hk, d = (case[n] for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim"))
+        for side in ("q", "kv"):
+            st[side + "_lens"] = _lengths(case, side)
+            total = torch.tensor(st[side + "_lens"], dtype=torch.int64).cumsum(0)
+            st[side + "_offset"] = total.to(torch.int32).to(DEV) if case["packed_" + side] else None
+            st[side + "_rows"] = int(total[-1])
+        qs = (st["q_rows"],) if case["packed_q"] else (b, lq)
+        ks = (st["kv_rows"],) if case["packed_kv"] else (b, lk)
+        st["q"] = _normal(g, *qs, h, d, scale=1.5).requires_grad_(case["train"])
+        st["k"] = _normal(g, *ks, hk, d).requires_grad_(case["train"])
+        st["v"] = _normal(g, *ks, hk, d).requires_grad_(case["train"])
+        st["mask"] = None
+        if case["masked"]:
+            mask = torch.rand(b, lk, generator=g, device=DEV) < 0.2
+            ends = torch.randint((lk + 1) // 2, lk + 1, (b, 1), generator=g, device=DEV)
+            mask |= torch.arange(lk, device=DEV)[None] >= ends
+            if b >= 3:
+                mask[1] = True  # a padded entry of the batch: nothing to read
+            st["mask"] = mask
+        if case["train"]:
+            st["dout"] = _normal(g, *qs, h, d)
+        return st
+    r, e, f, train = case["rows"], case["width"], case["hidden"], case["train"]
+    st["x"] = _normal(g, r, e).requires_grad_(train)
+    st["w_gate"] = _normal(g, f, e, scale=1.0 / math.sqrt(e)).requires_grad_(train)
+    st["w_up"] = _normal(g, f, e, scale=1.0 / math.sqrt(e)).requires_grad_(train)
+    st["w_down"] = _normal(g, e, f, scale=1.0 / math.sqrt(f)).requires_grad_(train)
+    if case["bias"]:
+        st["b_gate"] = _normal(g, f, scale=0.3).requires_grad_(train)
+        st["b_up"] = _normal(g, f, scale=0.3).requires_grad_(train)
+        st["b_down"] = _normal(g, e, scale=0.3).requires_grad_(train)
+    if train:
+        st["dout"] = _normal(g, r, e)
+    return st
+
+
+def _coords(g, t, axes, case):
+    if case["whole"]:
+        hi = case["far"] or 160
+        return torch.randint(0, hi, (t, axes), generator=g, device=DEV, dtype=torch.int32)
+    return (torch.rand(t, axes, generator=g, device=DEV) - 0.5) * 160.0  # a table-top of 0.8 m in voxels of 5 mm
+
+
+# ---- one pass ------------------------------------------------------------------------------------------------------------------
+
+def run(state):
+    case = state["case"]
+    if own:
+        return {"rotary": _own_rotary, "cross": _own_cross, "ffn": _own_ffn}[case["op"]](state, case)
+    with torch.no_grad():
+        return {"rotary": _plain_rotary, "cross": _plain_cross, "ffn": _plain_ffn}[case["op"]](state, case)
+
+
+BASE = 10000.0
+
+
+def _own_rotary(st, case):
+    from pointcloudmatters_amd.policy import rotary_axes
+
+    out = rotary_axes(st["x"], st["coords"], st["sections"], base=BASE, interleaved=case["interleaved"])
+    if not case["train"]:
+        return out
+    return [out, *torch.autograd.grad(out, (st["x"],), st["dout"])]
+
+
+def _own_cross(st, case):
+    from pointcloudmatters_amd.policy import cross_attention
+
+    out = cross_attention(st["q"], st["k"], st["v"], key_padding_mask=st["mask"], q_offset=st["q_offset"], kv_offset=st["kv_offset"])
+    if not case["train"]:
+        return out
+    return [out, *torch.autograd.grad(out, (st["q"], st["k"], st["v"]), st["dout"])]
+
+
+FFN_WEIGHTS = ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
+
+
+def _own_ffn(st, case):
+    from pointcloudmatters_amd.policy import gated_ffn
+
+    out = gated_ffn(st["x"], st["w_gate"], st["w_up"], st["w_down"], b_gate=st.get("b_gate"), b_up=st.get("b_up"),
+                    b_down=st.get("b_down"), activation=case["act"])
+    if not case["train"]:
+        return out
+    return [out, *torch.autograd.grad(out, [st[n] for n in FFN_WEIGHTS if n in st], st["dout"])]
+
+
+# ---- the plain forms: elementary operations in 32 bits ---------------------------------------------------------------------------
+
+def _frequencies(sections):
+    return torch.tensor([BASE ** (-j / n) for n in sections for j in range(n)], dtype=torch.float64, device=DEV)
+
+
+def _turn(x, cos, sin, half, interleaved):
+    """Pairs of the first 2 * half channels of x (T, H, D) turned by (cos, sin) (T, 1, half)."""
+    x = x.float()
+    a, b = (x[..., 0:2 * half:2], x[..., 1:2 * half:2]) if interleaved else (x[..., :half], x[..., half:2 * half])
+    u, v = a * cos - b * sin, a * sin + b * cos
+    turned = torch.stack((u, v), dim=-1).flatten(-2) if interleaved else torch.cat((u, v), dim=-1)
+    return torch.cat((turned, x[..., 2 * half:]), dim=-1)
+
+
+def _plain_rotary(st, case):
+    x, sections = st["x"], st["sections"]
+    axis = torch.repeat_interleave(torch.arange(len(sections), device=DEV), torch.tensor(sections, device=DEV), output_size=sum(sections))
+    angle = st["coords"].double()[:, axis] * _frequencies(sections)  # 64 bits: far positions lose their angle in 32
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+    out = _turn(x, cos, sin, sum(sections), case["interleaved"]).to(x.dtype)
+    if not case["train"]:
+        return out
+    return [out, _turn(st["dout"], cos, -sin, sum(sections), case["interleaved"]).to(x.dtype)]
+
+
+def _layout(st, side):
+    """Where a packed side's rows stand when every sequence is padded to the longest: (index of the row of each padded place (B, M),
+    which places hold a row (B, M), padded place of each row (rows,))."""
+    lens = torch.tensor(st[side + "_lens"], device=DEV)
+    most = max(max(st[side + "_lens"]), 1)
+    place = torch.arange(most, device=DEV)[None]
+    start = (lens.cumsum(0) - lens)[:, None]
+    held = place < lens[:, None]
+    index = torch.where(held, start + place, 0)
+    return index, held, held.flatten().nonzero_static(size=st[side + "_rows"]).flatten()
+
+
+def _heads_first(t, group):
+    """(B, M, H, D) -> (B * Hkv, group * M, D), the heads that share a key head side by side."""
+    b, m, h, d = t.shape
+    return t.view(b, m, h // group, group, d).permute(0, 2, 3, 1, 4).reshape(b * (h // group), group * m, d)
+
+
+def _heads_back(t, b, group):
+    n, gm, d = t.shape
+    return t.view(b, n // b, group, gm // group, d).permute(0, 3, 1, 2, 4).reshape(b, gm // group, n // b * group, d)
+
+
+def _plain_cross(st, case):
+    b, group, d = case["batch"], case["heads"] // case["kv_heads"], case["dim"]
+    scale = 1.0 / math.sqrt(d)
+    q, k, v, dout = (st.get(n) for n in ("q", "k", "v", "dout"))
+    seen = None
+    if case["packed_q"]:
+        qi, qheld, qplace = _layout(st, "q")
+        q = q[qi] if st["q_rows"] else q.new_zeros(b, 1, case["heads"], d)
+        dout = dout[qi] * qheld[..., None, None] if dout is not None else None
+    if case["packed_kv"]:
+        ki, seen, kplace = _layout(st, "kv")
+        k, v = k[ki], v[ki]
+    elif st["mask"] is not None:
+        seen = ~st["mask"]
+    qh, kh, vh = _heads_first(q.float(), group), _heads_first(k.float(), 1), _heads_first(v.float(), 1)
+    if seen is not None:
+        every = torch.repeat_interleave(seen, case["kv_heads"], dim=0, output_size=b * case["kv_heads"])
+        kh, vh = kh.masked_fill(~every[..., None], 0.0), vh.masked_fill(~every[..., None], 0.0)
+    s = torch.bmm(qh, kh.transpose(1, 2)).mul_(scale)
+    if seen is not None:
+        s.masked_fill_(~every[:, None], -math.inf)
+    top = s.amax(-1, keepdim=True).clamp_min_(torch.finfo(torch.float32).min)
+    p = s.sub_(top).exp_()
+    p /= p.sum(-1, keepdim=True).clamp_min_(torch.finfo(torch.float32).tiny)
+    o = _heads_back(torch.bmm(p, vh), b, group)
+    outs = [o.to(st["q"].dtype)]
+    if case["train"]:
+        do = _heads_first(dout.float(), group)
+        dv = torch.bmm(p.transpose(1, 2), do)
+        dp = torch.bmm(do, vh.transpose(1, 2))
+        dp -= (dp * p).sum(-1, keepdim=True)
+        ds = dp.mul_(p).mul_(scale)
+        dq, dk = torch.bmm(ds, kh), torch.bmm(ds.transpose(1, 2), qh)
+        outs += [_heads_back(dq, b, group).to(st["q"].dtype)] + [_heads_back(t, b, 1).to(st["q"].dtype) for t in (dk, dv)]
+    if case["packed_q"]:
+        outs[:2] = [t.flatten(0, 1)[qplace] for t in outs[:2]]
+    if case["packed_kv"]:
+        outs[2:] = [t.flatten(0, 1)[kplace] for t in outs[2:]]
+    return outs if case["train"] else outs[0]
+
+
+def _act(a, kind):
+    """act(a) and act'(a)."""
+    if kind == "silu":
+        s = torch.sigmoid(a)
+        return a * s, s * (1.0 + a * (1.0 - s))
+    if kind == "gelu":
+        c = 0.5 * (1.0 + torch.erf(a * math.sqrt(0.5)))
+        return a * c, c + a * torch.exp(-0.5 * a * a) * (1.0 / math.sqrt(2.0 * math.pi))
+    return a.clamp_min(0.0), (a > 0).to(a.dtype)
+
+
+def _plain_ffn(st, case):
+    x, wg, wu, wd = (st[n].float() for n in ("x", "w_gate", "w_up", "w_down"))
+    a, u = x @ wg.t(), x @ wu.t()
+    if case["bias"]:
+        a += st["b_gate"].float()
+        u += st["b_up"].float()
+    s, ds = _act(a, case["act"])
+    h = s * u
+    y = h @ wd.t()
+    if case["bias"]:
+        y += st["b_down"].float()
+    if not case["train"]:
+        return y.to(st["x"].dtype)
+    dy = st["dout"].float()
+    dh = dy @ wd
+    da, du = dh * u * ds, dh * s
+    outs = [y, da @ wg + du @ wu, da.t() @ x, du.t() @ x, dy.t() @ h]
+    if case["bias"]:
+        outs += [da.sum(0), du.sum(0), dy.sum(0)]
+    return [t.to(st["x"].dtype) for t in outs]
+
+
+# ---- the work of a pass ----------------------------------------------------------------------------------------------------------
+
+def work(case):
+    """Every input read once, every output written once; the multiplications and additions of the products."""
+    t = case["train"]
+    if case["op"] == "rotary":
+        values = case["rows"] * case["heads"] * case["dim"]
+        size = 2 if case["dtype"] == "bf16" else 4
+        axes = len(case["sections"].split(","))
+        return {"bytes": 2 * values * size * (2 if t else 1) + 4 * case["rows"] * axes, "flops": 3 * values * (2 if t else 1)}
+    if case["op"] == "cross":
+        h, hk, d = case["heads"], case["kv_heads"], case["dim"]
+        lq, lk = _lengths(case, "q"), _lengths(case, "kv")
+        if case["masked"]:  # a fifth of the keys is masked, and all behind the padded ends: 0.6 of them are left on average
+            lk = [0 if i == 1 and case["batch"] >= 3 else 0.6 * n for i, n in enumerate(lk)]
+        rows, cells = 2 * sum(lq) * h * d, 4 * sum(lk) * hk * d  # bytes of q (or of the output), of k and v together
+        products = 2 * h * d * sum(a * c for a, c in zip(lq, lk))
+        return {"bytes": int(4 * rows + 2 * cells if t else 2 * rows + cells), "flops": int(products * (7 if t else 2))}
+    r, e, f = case["rows"], case["width"], case["hidden"]
+    return {"bytes": 2 * ((4 * r * e + 6 * e * f) if t else (2 * r * e + 3 * e * f)), "flops": 6 * r * e * f * (3 if t else 1)}
+
+
+# ---- the definitions in 64 bits ----------------------------------------------------------------------------------------------------
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    with torch.no_grad():
+        return {"rotary": _exact_rotary, "cross": _exact_cross, "ffn": _exact_ffn}[case["op"]](st, case)
+
+
+def _exact_rotary(st, case):
+    """Each pair as a complex number times exp(i angle)."""
+    sections, half = st["sections"], sum(st["sections"])
+    turn = []
+    for a, n in enumerate(sections):
+        step = torch.exp(torch.arange(n, dtype=torch.float64, device=DEV) * (-math.log(BASE) / n))
+        turn.append(st["coords"][:, a, None].to(torch.float64) * step)
+    turn = torch.polar(torch.ones((), dtype=torch.float64, device=DEV), torch.cat(turn, 1))[:, None]
+
+    def apply(x, w):
+        y = x.to(torch.float64).clone()
+        if case["interleaved"]:
+            first, second = slice(0, 2 * half, 2), slice(1, 2 * half, 2)
+        else:
+            first, second = slice(0, half), slice(half, 2 * half)
+        z = torch.complex(y[..., first].contiguous(), y[..., second].contiguous()) * w
+        y[..., first], y[..., second] = z.real, z.imag
+        return y
+
+    out = apply(st["x"], turn)
+    return [out, apply(st["dout"], turn.conj())] if case["train"] else out
+
+
+def _exact_cross(st, case):
+    """Sequence by sequence and head by head, only the keys that are there."""
+    d, group = case["dim"], case["heads"] // case["kv_heads"]
+    q, k, v = (st[n].detach() for n in ("q", "k", "v"))
+    out = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    dq, dk, dv = out.clone(), torch.zeros(k.shape, dtype=torch.float64, device=DEV), torch.zeros(k.shape, dtype=torch.float64, device=DEV)
+    q0 = k0 = 0
+    for i in range(case["batch"]):
+        ql, kl = st["q_lens"][i], st["kv_lens"][i]
+        qs, ks = slice(q0, q0 + ql), slice(k0, k0 + kl)
+        q0, k0 = q0 + ql, k0 + kl
+        qi, oi, dqi = (t[qs] if case["packed_q"] else t[i] for t in (q, out, dq))
+        ki, vi, dki, dvi = (t[ks] if case["packed_kv"] else t[i] for t in (k, v, dk, dv))
+        held = torch.arange(kl, device=DEV) if st["mask"] is None else (~st["mask"][i]).nonzero().flatten()
+        if ql == 0 or held.numel() == 0:
+            continue
+        for h in range(case["heads"]):
+            kk, vv, qq = ki[held, h // group].double(), vi[held, h // group].double(), qi[:, h].double()
+            p = torch.softmax(qq @ kk.T / math.sqrt(d), dim=-1)
+            oi[:, h] = p @ vv
+            if case["train"]:
+                g = (st["dout"][qs] if case["packed_q"] else st["dout"][i])[:, h].double()
+                ds = p * (g @ vv.T - (g * oi[:, h]).sum(-1, keepdim=True)) / math.sqrt(d)
+                dqi[:, h] = ds @ kk
+                dki[held, h // group] += ds.T @ qq
+                dvi[held, h // group] += p.T @ g
+    return [out, dq, dk, dv] if case["train"] else out
+
+
+def _exact_ffn(st, case):
+    """The block from its definition, its gradients by differentiation."""
+    names = [n for n in FFN_WEIGHTS if n in st]
+    with torch.enable_grad():
+        t = {n: st[n].detach().double().requires_grad_(case["train"]) for n in names}
+        a, u = torch.addmm(t["b_gate"], t["x"], t["w_gate"].T) if case["bias"] else t["x"] @ t["w_gate"].T, t["x"] @ t["w_up"].T
+        if case["bias"]:
+            u = u + t["b_up"]
+        if case["act"] == "silu":
+            s = a / (1.0 + torch.exp(-a))
+        elif case["act"] == "gelu":
+            s = 0.5 * a * torch.erfc(-a / math.sqrt(2.0))
+        else:
+            s = torch.relu(a)
+        y = (s * u) @ t["w_down"].T
+        if case["bias"]:
+            y = y + t["b_down"]
+        if not case["train"]:
+            return y.detach()
+        return [y.detach(), *torch.autograd.grad(y, [t[n] for n in names], st["dout"].double())]
