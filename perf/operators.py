@@ -77,13 +77,14 @@ def draw(rng):
             sections.append(n)
             left -= n
         whole = rng.random() < 0.5
-        return dict(op="rotary", rows=_log(rng, 1, 120e6 / (heads * dim)), heads=heads, dim=dim, sections=",".join(map(str, sections)),
+        return dict(op="rotary", rows=_log(rng, 1, 60e6 / (heads * dim)), heads=heads, dim=dim, sections=",".join(map(str, sections)),
                     dtype=rng.choice(["bf16", "fp32"]), whole=whole, far=rng.choice([0, 1 << 20]) if whole else 0,
                     interleaved=rng.random() < 0.5, train=rng.random() < 0.5)
     if op == "cross":
         heads, kv_heads = rng.choice([(8, 8), (4, 4), (8, 2), (16, 4), (6, 2), (5, 1), (16, 16)])
         dim, train = rng.choice([32, 64, 64, 80, 128]), rng.random() < 0.5
-        batch, keys = _log(rng, 1, 32), _log(rng, 16 if train else 1, 16384)  # one key alone has no gradient to compare: its weight is 1
+        batch = _log(rng, 1, 32)  # one key alone has no gradient to compare (its weight is 1), so a training step has 16 at least
+        keys = _log(rng, 16 if train else 1, min(16384, 1.0e8 / (batch * kv_heads * dim)))
         most = 1.2e11 / (4 * batch * heads * dim * keys * (3.5 if train else 1))
         most = min(most, 1.0e9 / (batch * heads * keys), 1.0e8 / (batch * heads * dim), 2048)
         packed = rng.random() < 0.5
