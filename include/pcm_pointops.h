@@ -671,6 +671,51 @@ int pcm_adamw_flat_hip(long n, float *p, const float *g, float *m, float *v, con
 #define PCM_XFER_COPY_2B 5
 int pcm_xfer_batch_hip(int n, void *const *dst, const void *const *src, const long *numel, const int *kind, void *stream);
 
+/* ---- rotary positions over several axes (csrc/rotary.hip) -------------------------------------------------------
+ * Pair j (of sections[a]) of axis a turns by coords[.., a] * base^(-j / sections[a]) radians; half = sum of sections; pairs are channels
+ * (i, i + half), or (2i, 2i + 1) when interleaved; channels from 2 half on are copied.  x / out: (B, L, H, D) of bf16 or fp32 at element
+ * strides (bs, ls, hs), channels contiguous; out == x with the same strides is allowed.  coords: (B, L, axes) at strides (c_bs, c_ls);
+ * coords_type 0 fp32, 1 int32, 2 int64.  sections: HOST array, axes <= 8, half <= 128, 2 half <= D.  inverse != 0 turns back (the
+ * gradient).  Angles are formed in fp64. */
+int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, const void *x, long x_bs, long x_ls, long x_hs, void *out,
+                        long o_bs, long o_ls, long o_hs, int coords_type, const void *coords, long c_bs, long c_ls, int axes,
+                        const int *sections, double base, int interleaved, int inverse, void *stream);
+
+/* ---- cross attention to states of another length (csrc/cross_attn.hip) -------------------------------------------
+ * out = softmax(scale q k^T) v per head, bf16, head h of H reads key head h / (H / Hkv); D a multiple of 8 up to 128.
+ * Each side is padded (offset NULL: B sequences of L resp. S rows at the batch stride) or packed (offset: B cumulative ends on the
+ * device; q_rows resp. kv_rows = all rows; the batch stride is ignored).  Strides (bs, ls, hs) in elements, multiples of 8; pointers
+ * 16-byte aligned.  mask (nullable): bytes, != 0 = ignore the key; (B, S) at mask_bs, or (kv_rows) for a packed side.  out, dq:
+ * (q rows, H, D) contiguous; dk, dv: (kv rows, Hkv, D) contiguous; lse (nullable in the forward), delta: (q rows, H) fp32.  A row without
+ * a key: out = 0, lse = -inf, dq = 0.  Rows of a packed side behind the last sequence: 0 as well.  Offsets are clamped to the row count.
+ * ws: pcm_cross_attn_ws_bytes bytes (0: none needed), 16-byte aligned, for either direction.  No atomics: results are reproducible. */
+int pcm_cross_attn_supported(int H, int Hkv, int D);
+long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed);
+int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
+                               const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
+                               long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,
+                               long mask_bs, float scale, void *out, float *lse, void *ws, long ws_bytes, void *stream);
+int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
+                                const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
+                                long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,
+                                long mask_bs, float scale, const void *out, const float *lse, const void *dout, long g_bs, long g_ls,
+                                long g_hs, float *delta, void *dq, void *dk, void *dv, void *ws, long ws_bytes, void *stream);
+
+/* ---- gated feed-forward block (csrc/gated_ffn.hip) ------------------------------------------------------------------
+ * y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd; bf16; x (R, E) at row stride x_ls, wg / wu (F, E), wd (E, F) contiguous, biases
+ * nullable; act 0 SiLU, 1 GELU (erf), 2 ReLU; any E and F.  y (R, E) contiguous.  h (R, Fp) and, for a backward pass, a, u (R, Fp; both or
+ * neither): the hidden values and the two projections at Fp = pcm_gated_ffn_hidden_ld(F) values a row, 16-byte aligned.
+ * Backward: gradients that are NULL are not computed (dwg with dwu, dbg with dbu).  ws: pcm_gated_ffn_ws_bytes bytes, 16-byte aligned.
+ * No atomics: results are reproducible. */
+long pcm_gated_ffn_hidden_ld(int F);
+long pcm_gated_ffn_ws_bytes(long R, int E, int F, int backward);
+int pcm_gated_ffn_forward_hip(long R, int E, int F, int act, const void *x, long x_ls, const void *wg, const void *wu, const void *wd,
+                              const void *bg, const void *bu, const void *bd, void *y, void *a, void *u, void *h, void *ws,
+                              long ws_bytes, void *stream);
+int pcm_gated_ffn_backward_hip(long R, int E, int F, int act, const void *x, long x_ls, const void *wg, const void *wu, const void *wd,
+                               const void *a, const void *u, const void *h, const void *dy, long dy_ls, void *dx, void *dwg, void *dwu,
+                               void *dwd, void *dbg, void *dbu, void *dbd, void *ws, long ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

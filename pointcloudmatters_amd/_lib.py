@@ -15,6 +15,7 @@ CSRC_DIR = os.path.join(_HERE, "csrc")
 _P = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_l = ctypes.c_long
 
 # name -> argtypes, exactly the declarations of include/pcm_pointops.h (stream last, as void*)
 SIGNATURES = {
@@ -151,11 +152,26 @@ SIGNATURES = {
     "pcm_grad_sumsq_hip": [ctypes.c_long, _P, _P, _P, _P],
     "pcm_adamw_flat_hip": [ctypes.c_long, _P, _P, _P, _P, _P, _P, _i, _P, _P, _P],
     "pcm_xfer_batch_hip": [_i, _P, _P, _P, _P, _P],
+    # B, L, H, D, x_is_bf16, x + 3 strides, out + 3 strides, coords_type, coords + 2 strides, axes, sections, base, interleaved, inverse, stream
+    "pcm_rotary_axes_hip": [_l, _l, _i, _i, _i, _P, _l, _l, _l, _P, _l, _l, _l, _i, _P, _l, _l, _i, _P, ctypes.c_double, _i, _i, _P],
+    "pcm_cross_attn_supported": [_i, _i, _i],
+    "pcm_cross_attn_ws_bytes": [_i, _i, _i, _i, _i, _l, _i, _i, _l, _i],
+    # B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset, (q, k, v) + 3 strides each, mask, mask_bs, scale, out, lse, ws, ws_bytes, stream
+    "pcm_cross_attn_forward_hip": [_i, _i, _i, _i, _i, _l, _P, _i, _l, _P] + 3 * [_P, _l, _l, _l] + [_P, _l, _f, _P, _P, _P, _l, _P],
+    # ..., scale, out, lse, dout + 3 strides, delta, dq, dk, dv, ws, ws_bytes, stream
+    "pcm_cross_attn_backward_hip": [_i, _i, _i, _i, _i, _l, _P, _i, _l, _P] + 3 * [_P, _l, _l, _l] + [_P, _l, _f, _P, _P, _P, _l, _l, _l]
+    + 5 * [_P] + [_l, _P],
+    "pcm_gated_ffn_hidden_ld": [_i],
+    "pcm_gated_ffn_ws_bytes": [_l, _i, _i, _i],
+    # R, E, F, act, x, x_ls, wg, wu, wd, bg, bu, bd, y, a, u, h, ws, ws_bytes, stream
+    "pcm_gated_ffn_forward_hip": [_l, _i, _i, _i, _P, _l] + 11 * [_P] + [_l, _P],
+    # R, E, F, act, x, x_ls, wg, wu, wd, a, u, h, dy, dy_ls, dx, dwg, dwu, dwd, dbg, dbu, dbd, ws, ws_bytes, stream
+    "pcm_gated_ffn_backward_hip": [_l, _i, _i, _i, _P, _l] + 7 * [_P] + [_l] + 8 * [_P] + [_l, _P],
 }
 
 # functions that return a size (long); everything else returns an int status
 LONG_RESULTS = ("pcm_scatter_plan_ws_ints", "pcm_scatter_plan_sorted_scratch_ints", "pcm_sa_index_det_scratch_ints",
-                "pcm_sa_bwd1_det_ws_bytes", "pcm_ball_query_ws_bytes")
+                "pcm_sa_bwd1_det_ws_bytes", "pcm_ball_query_ws_bytes", "pcm_cross_attn_ws_bytes", "pcm_gated_ffn_hidden_ld", "pcm_gated_ffn_ws_bytes")
 
 _LIB = None
 

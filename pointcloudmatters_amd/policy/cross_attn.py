@@ -1,0 +1,146 @@
+"""Attention of queries over an encoder's states of another length (csrc/cross_attn.hip): the clouds of a batch side by side in the
+packed layout of the point ops (one cumulative `offset` per cloud) or padded with a mask, shared key heads, head widths up to 128, one
+query or thousands.  Stands beside `small_attn.small_attention`, which takes padded (B, L, E) tensors with heads of 64.
+"""
+import math
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .. import _graphs, _lib
+from ..pointops import _common
+from .._lib import raw_stream as _raw_stream
+
+MAX_HEAD_DIM = 128
+
+
+def _fit(t):
+    """t, or a contiguous copy where the kernels' 16-byte accesses do not fit its strides or address."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(st % 8 == 0 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t):
+    """(batch, row, head) strides in elements; 0 where there is one entry only."""
+    st = [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+    return tuple(st) if t.dim() == 4 else (0, *st)
+
+
+def _sides(q, k, q_offset, kv_offset):
+    """The leading arguments that describe both sides, (B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset)."""
+    b = q.shape[0] if q.dim() == 4 else q_offset.numel()
+    return (b, q.shape[-2], k.shape[-2], q.shape[-1], q.shape[1] if q.dim() == 4 else 0, math.prod(q.shape[:-2]),
+            q_offset.data_ptr() if q.dim() == 3 else 0, k.shape[1] if k.dim() == 4 else 0, math.prod(k.shape[:-2]),
+            kv_offset.data_ptr() if k.dim() == 3 else 0)
+
+
+def _workspace(L_, sides, dev):
+    b, h, hkv, d, l, q_rows, qo, s, kv_rows, ko = sides
+    n = L_.pcm_cross_attn_ws_bytes(b, h, hkv, d, l, q_rows, int(qo != 0), s, kv_rows, int(ko != 0))
+    return torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _operands(q, k, v, mask, scale):
+    mask_bs = mask.stride(0) if mask is not None and mask.dim() == 2 else 0
+    return (q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), _ptr(mask), mask_bs, scale)
+
+
+class _CrossAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, q_offset, kv_offset, scale, want_lse):
+        L_ = _lib.load()
+        q, k, v = _fit(q), _fit(k), _fit(v)
+        dev = q.device
+        grad = any(ctx.needs_input_grad[:3])
+        with torch.cuda.device(dev):
+            sides = _sides(q, k, q_offset, kv_offset)
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if grad or want_lse else None
+            ws = _workspace(L_, sides, dev)
+            rc = L_.pcm_cross_attn_forward_hip(*sides, *_operands(q, k, v, mask, scale), out.data_ptr(), _ptr(lse), _ptr(ws),
+                                               ws.numel() * 4 if ws is not None else 0, _raw_stream())
+        _lib.check(rc, "pcm_cross_attn_forward_hip")
+        if lse is not None:
+            ctx.mark_non_differentiable(lse)
+        if grad:
+            ctx.save_for_backward(q, k, v, mask, q_offset, kv_offset, out, lse)
+            ctx.scale = scale
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, _):
+        L_ = _lib.load()
+        q, k, v, mask, q_offset, kv_offset, out, lse = ctx.saved_tensors
+        dout = _fit(dout)
+        dev = q.device
+        with torch.cuda.device(dev):
+            sides = _sides(q, k, q_offset, kv_offset)
+            dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2))
+            delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
+            ws = _workspace(L_, sides, dev)
+            rc = L_.pcm_cross_attn_backward_hip(*sides, *_operands(q, k, v, mask, ctx.scale), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                                *_strides(dout), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws),
+                                                ws.numel() * 4 if ws is not None else 0, _raw_stream())
+        _lib.check(rc, "pcm_cross_attn_backward_hip")
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _check_offset(offset, side, t, name):
+    if t.dim() == 4:
+        if offset is not None:
+            raise ValueError("cross_attention: %s is padded (4 dimensions): it takes no %s_offset" % (name, side))
+        return None
+    if offset is None:
+        raise ValueError("cross_attention: packed %s (3 dimensions) needs %s_offset" % (name, side))
+    if offset.dim() != 1 or offset.numel() < 1 or offset.is_floating_point() or offset.device != t.device:
+        raise ValueError("cross_attention: %s_offset must be a 1-d integer tensor on %s" % (side, t.device))
+    return _common.i32c(offset)
+
+
+def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=None, scale=None, return_lse=False):
+    """softmax(scale * q k^T) v per head; q, k, v bfloat16.
+
+    q: (B, L, H, D), or packed (T, H, D) with `q_offset`; k, v: (B, S, Hkv, D), or packed (T', Hkv, D) with `kv_offset`.  An offset is
+    the int tensor (B,) of the point ops: sequence b holds rows [offset[b - 1], offset[b]).  H is a multiple of Hkv (query head h reads
+    key head h // (H / Hkv)); D a multiple of 8 up to 128; any strides with the channels contiguous (what 16-byte accesses do not fit is
+    copied first).  key_padding_mask: bool (B, S), or (T',) for packed keys, True = ignore (the nn.MultiheadAttention convention);
+    whatever stands in masked or absent rows, NaN and infinities included, has no influence.  scale: > 0, 1 / sqrt(D) by default.
+
+    Returns (.., H, D) like q; a row without a key is zero, so are packed rows behind the last sequence.  return_lse: also the natural
+    logarithm of each row's sum of exponentials, fp32, q.shape[:-1] (-inf without a key; no gradient).  Gradients for q, k and v; results
+    do not change from run to run (no atomics)."""
+    _common.require_hip(q, k, v, key_padding_mask, q_offset, kv_offset)
+    if q.dim() not in (3, 4) or k.dim() not in (3, 4) or v.shape != k.shape:
+        raise ValueError("cross_attention: shapes q %s, k %s, v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+        raise TypeError("cross_attention: q, k, v must be bfloat16, got %s, %s, %s" % (q.dtype, k.dtype, v.dtype))
+    if not q.device == k.device == v.device:
+        raise ValueError("cross_attention: q, k, v are on %s, %s, %s" % (q.device, k.device, v.device))
+    h, d = q.shape[-2:]
+    hkv = k.shape[-2]
+    if k.shape[-1] != d or hkv < 1 or h < 1 or h % hkv:
+        raise ValueError("cross_attention: %d heads of %d over %d key heads of %d" % (h, d, hkv, k.shape[-1]))
+    if d % 8 or not 8 <= d <= MAX_HEAD_DIM:
+        raise ValueError("cross_attention: head width %d is not a multiple of 8 up to %d" % (d, MAX_HEAD_DIM))
+    q_offset, kv_offset = _check_offset(q_offset, "q", q, "q"), _check_offset(kv_offset, "kv", k, "k / v")
+    b = q.shape[0] if q.dim() == 4 else q_offset.numel()
+    if (k.shape[0] if k.dim() == 4 else kv_offset.numel()) != b:
+        raise ValueError("cross_attention: %d query sequences, %d key sequences" % (b, k.shape[0] if k.dim() == 4 else kv_offset.numel()))
+    mask = key_padding_mask
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.shape != k.shape[:-2] or mask.device != k.device:
+            raise ValueError("cross_attention: key_padding_mask must be a bool tensor %s on %s" % (tuple(k.shape[:-2]), k.device))
+        mask = mask.contiguous().view(torch.uint8)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("cross_attention: scale must be positive and finite, got %r" % (scale,))
+    out, lse = _CrossAttention.apply(q, k, v, mask, q_offset, kv_offset, scale, bool(return_lse))
+    _graphs.guard_leaves(out, "cross_attention")
+    return (out, lse) if return_lse else out

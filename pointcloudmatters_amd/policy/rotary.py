@@ -1,0 +1,78 @@
+"""Rotary positions over several axes (csrc/rotary.hip): the turn of a token's head channels by its own coordinates -- x, y, z of a
+point, or time, height and width of a frame -- that makes q . k depend on the difference of two tokens' positions.  Stands beside the
+additive embedding `sa_layer.coord_embedding_sine`; applied to the queries and the keys in front of an attention.
+"""
+import ctypes
+
+import torch
+from torch.autograd import Function
+
+from .. import _graphs, _lib
+from ..pointops import _common
+from .._lib import raw_stream as _raw_stream
+
+MAX_PAIRS = 128  # turned pairs of a head
+MAX_AXES = 8
+_COORDS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+
+
+def _launch(x, coords, sections, base, interleaved, inverse):
+    L_ = _lib.load()
+    x = x if x.stride(-1) == 1 else x.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    lead = x.shape[:-2]
+    b, l = (1, lead[0]) if len(lead) == 1 else lead
+    xs = (0, *x.stride()[:2]) if len(lead) == 1 else x.stride()[:3]
+    os_ = (0, *out.stride()[:2]) if len(lead) == 1 else out.stride()[:3]
+    c_bs = coords.stride(0) if coords.dim() == 3 else 0
+    with torch.cuda.device(x.device):
+        rc = L_.pcm_rotary_axes_hip(b, l, x.shape[-2], x.shape[-1], int(x.dtype == torch.bfloat16), x.data_ptr(), *xs, out.data_ptr(), *os_,
+                                    _COORDS[coords.dtype], coords.data_ptr(), c_bs, coords.stride(-2), len(sections),
+                                    (ctypes.c_int * len(sections))(*sections), float(base), int(interleaved), int(inverse), _raw_stream())
+    _lib.check(rc, "pcm_rotary_axes_hip")
+    return out
+
+
+class _RotaryAxes(Function):
+    @staticmethod
+    def forward(ctx, x, coords, sections, base, interleaved):
+        ctx.save_for_backward(coords)
+        ctx.meta = (sections, base, interleaved)
+        return _launch(x, coords, sections, base, interleaved, False)
+
+    @staticmethod
+    def backward(ctx, dout):
+        (coords,) = ctx.saved_tensors
+        return _launch(dout, coords, *ctx.meta, True), None, None, None, None
+
+
+def rotary_axes(x, coords, sections, base=10000.0, interleaved=False):
+    """x (T, H, D) or (B, L, H, D), bf16 or fp32, turned by coords (T, A) / (B, L, A) / (L, A) (fp32, int32 or int64; one row for all
+    heads of a token).  sections: A pair counts; pair j of axis a turns by ``coords[..., a] * base ** (-j / sections[a])`` radians.  With
+    half = sum(sections) the pairs are channels (i, i + half), or (2 i, 2 i + 1) when `interleaved`; channels from 2 * half on pass
+    through.  Any strides with the channels contiguous.  Returns a new contiguous tensor of x's type (fp32 arithmetic; angles in fp64,
+    off by about 2^-52 of themselves: less than fp32 resolves up to 2^26 radians); x gets a gradient, coords must not ask for one."""
+    _common.require_hip(x, coords)
+    sections = tuple(int(n) for n in sections)
+    if x.dim() not in (3, 4):
+        raise ValueError("rotary_axes: x must be (T, H, D) or (B, L, H, D), got %s" % (tuple(x.shape),))
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("rotary_axes: x must be bfloat16 or float32, got %s" % x.dtype)
+    if coords.dtype not in _COORDS:
+        raise TypeError("rotary_axes: coords must be float32, int32 or int64, got %s" % coords.dtype)
+    if coords.requires_grad:
+        raise ValueError("rotary_axes: coords get no gradient: detach them")
+    if coords.device != x.device:
+        raise ValueError("rotary_axes: x is on %s, coords on %s" % (x.device, coords.device))
+    lead = tuple(x.shape[:-2])
+    if coords.dim() < 2 or tuple(coords.shape[:-1]) not in (lead, lead[-1:]):
+        raise ValueError("rotary_axes: coords %s do not fit x %s" % (tuple(coords.shape), tuple(x.shape)))
+    if not 1 <= len(sections) <= MAX_AXES or coords.shape[-1] != len(sections):
+        raise ValueError("rotary_axes: %d sections for %d coordinates (at most %d)" % (len(sections), coords.shape[-1], MAX_AXES))
+    half = sum(sections)
+    if min(sections) < 0 or not 1 <= half <= MAX_PAIRS or 2 * half > x.shape[-1]:
+        raise ValueError("rotary_axes: sections %s turn %d channels of a head of %d (at most %d)" % (sections, 2 * half, x.shape[-1], 2 * MAX_PAIRS))
+    if not base > 0:
+        raise ValueError("rotary_axes: base must be positive, got %r" % (base,))
+    coords = coords if coords.stride(-1) == 1 else coords.contiguous()
+    return _graphs.guard_leaves(_RotaryAxes.apply(x, coords, sections, float(base), bool(interleaved)), "rotary_axes")

@@ -51,7 +51,7 @@ CLANG = os.environ.get("WAVESIM_CXX", "/opt/rocm/lib/llvm/bin/clang++")
 # every kernel file of the library except graph_fix.hip (hipGraph surgery: runtime API, no kernel logic)
 SOURCES = ["fps.hip", "knn.hip", "ball.hip", "group.hip", "misc_ops.hip", "segsum.hip", "voxel.hip", "sa_scatter.hip", "sa_fused.hip",
            "bnrelu.hip", "drln.hip", "tokens.hip", "gnmish.hip", "ddpm.hip", "optim.hip", "ffn.hip", "ffn_mfma.hip", "attn_small.hip",
-           "attn_flash.hip", "proj_ln.hip"] + ([] if VARIANT == "next" else ["bnact.hip"])  # next/bnrelu.hip exports the pcm_bn_act_* entry points itself
+           "attn_flash.hip", "proj_ln.hip", "rotary.hip", "cross_attn.hip", "gated_ffn.hip"] + ([] if VARIANT == "next" else ["bnact.hip"])  # next/bnrelu.hip exports the pcm_bn_act_* entry points itself
 
 
 def source_path(name):
