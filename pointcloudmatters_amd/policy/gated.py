@@ -18,7 +18,7 @@ def _ptr(t):
 
 def _workspace(L_, rows, e, f, backward, dev):
     n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, int(backward))
-    return n, torch.empty(n, dtype=torch.uint8, device=dev)
+    return n, (torch.empty(n, dtype=torch.uint8, device=dev) if n else None)
 
 
 def _rows(t, width):
@@ -43,7 +43,7 @@ class _GatedFFN(Function):
             n, ws = _workspace(L_, rows, e, f, False, x.device)
             rc = L_.pcm_gated_ffn_forward_hip(rows, e, f, act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                                               _ptr(b_gate), _ptr(b_up), _ptr(b_down), y.data_ptr(), _ptr(a), _ptr(u), h.data_ptr(),
-                                              ws.data_ptr(), n, _raw_stream())
+                                              _ptr(ws), n, _raw_stream())
         _lib.check(rc, "pcm_gated_ffn_forward_hip")
         if grad:
             ctx.save_for_backward(x, w_gate, w_up, w_down, a, u, h)
@@ -68,7 +68,7 @@ class _GatedFFN(Function):
             n, ws = _workspace(L_, rows, e, f, True, dev)
             rc = L_.pcm_gated_ffn_backward_hip(rows, e, f, ctx.act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
                                                w_down.data_ptr(), a.data_ptr(), u.data_ptr(), h.data_ptr(), dy.data_ptr(), dy.stride(0),
-                                               _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), ws.data_ptr(), n,
+                                               _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), _ptr(ws), n,
                                                _raw_stream())
         _lib.check(rc, "pcm_gated_ffn_backward_hip")
         return (dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dbg if need[4] else None, dbu if need[5] else None, dbd, None)

@@ -153,7 +153,7 @@ def test_entry_points_reject_before_they_touch_the_runtime():
     assert L.pcm_cross_attn_supported(8, 2, 64) == 1 and L.pcm_cross_attn_supported(8, 3, 64) == 0 and L.pcm_cross_attn_supported(8, 2, 4) == 0
     assert L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 5, 5, 0) == 0 < L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 100000, 100000, 0)
 
-    def ff(R=4, E=16, F=8, act=0, x=p, a=None, u=None, h=p, ws=p, wsb=1 << 30):
+    def ff(R=40, E=16, F=8, act=0, x=p, a=None, u=None, h=p, ws=p, wsb=1 << 30):
         return L.pcm_gated_ffn_forward_hip(R, E, F, act, x, E, p, p, p, None, None, None, p, a, u, h, ws, wsb, None)
 
     assert ff(act=3) == 1 and ff(act=-1) == 1 and ff(x=None) == 1 and ff(a=p) == 1 and ff(h=None) == 1 and ff(h=0x1002) == 1 and ff(E=0) == 1

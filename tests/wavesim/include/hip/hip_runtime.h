@@ -157,6 +157,10 @@ template <class P> inline __attribute__((always_inline)) ws_s4 ws_ds_read_tr16(P
 }
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) ws_ds_read_tr16((p), WS_SITE)
 
+// global_load_lds: lane i's `size` bytes go to the (wave-uniform) LDS base + i * size
+#define __builtin_amdgcn_global_load_lds(g, l, size, off, aux) \
+    std::memcpy((char *)(void *)(l) + (off) + (size) * wavesim::g_cur->lane, (const char *)(const void *)(g) + (off), (size))
+
 // matrix instructions: every lane deposits its operand registers, the resolver multiplies with the ISA's operand layouts (wavesim.cpp)
 typedef float ws_f16v __attribute__((ext_vector_type(16)));
 typedef float ws_f4v __attribute__((ext_vector_type(4)));
