@@ -2,6 +2,7 @@
 ``include/pcm_pointops.h``.  There is NO fallback: if the library is missing or a symbol is absent
 the import of any product op raises, and every op refuses non-HIP tensors.
 """
+import contextlib
 import ctypes
 import os
 import subprocess
@@ -240,6 +241,15 @@ def raw_stream():
     `torch.cuda.current_stream().cuda_stream`, builds a Stream object and costs ~13 us per call -- 0.2 ms per training step
     over the eager launches of hybrid mode (tools/dbg/host_profile.py); this is one C call."""
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(device):
+    """`with on_device(t.device):` -- torch.cuda.device(device), without its two device queries when that is the current one already
+    (3 us of a small operator's call)."""
+    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def copy_batch(pairs):

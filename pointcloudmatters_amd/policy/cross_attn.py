@@ -16,80 +16,73 @@ MAX_HEAD_DIM = 128
 
 
 def _fit(t):
-    """t, or a contiguous copy where the kernels' 16-byte accesses do not fit its strides or address."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(st % 8 == 0 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    """(t, (batch, row, head) strides in elements, 0 where there is one entry only); t a contiguous copy where the kernels' 16-byte
+    accesses do not fit its strides or address."""
+    *st, last = t.stride()
+    if last != 1 or t.data_ptr() % 16 or any(s % 8 for s in st):
+        st = [s if n > 1 else 0 for s, n in zip(st, t.shape)]
+        if last != 1 or t.data_ptr() % 16 or any(s % 8 for s in st):
+            t = t.clone(memory_format=torch.contiguous_format)
+            st = t.stride()[:-1]
+    return t, (st if len(st) == 3 else (0, *st))
 
 
-def _strides(t):
-    """(batch, row, head) strides in elements; 0 where there is one entry only."""
-    st = [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
-    return tuple(st) if t.dim() == 4 else (0, *st)
+def _new(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _sides(q, k, q_offset, kv_offset):
-    """The leading arguments that describe both sides, (B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset)."""
-    b = q.shape[0] if q.dim() == 4 else q_offset.numel()
-    return (b, q.shape[-2], k.shape[-2], q.shape[-1], q.shape[1] if q.dim() == 4 else 0, math.prod(q.shape[:-2]),
-            q_offset.data_ptr() if q.dim() == 3 else 0, k.shape[1] if k.dim() == 4 else 0, math.prod(k.shape[:-2]),
-            kv_offset.data_ptr() if k.dim() == 3 else 0)
+def _arguments(q, k, v, mask, q_offset, kv_offset, scale):
+    """The operands as the kernels take them, the arguments that describe them, and the bytes of workspace of either direction."""
+    (q, qs), (k, ks), (v, vs) = _fit(q), _fit(k), _fit(v)
+    qshape, kshape = q.shape, k.shape
+    h, d, hkv = qshape[-2], qshape[-1], kshape[-2]
+    b, l, q_rows, qo = (qshape[0], qshape[1], qshape[0] * qshape[1], 0) if len(qshape) == 4 else (q_offset.numel(), 0, qshape[0], q_offset.data_ptr())
+    s, kv_rows, ko = (kshape[1], kshape[0] * kshape[1], 0) if len(kshape) == 4 else (0, kshape[0], kv_offset.data_ptr())
+    args = (b, h, hkv, d, l, q_rows, qo, s, kv_rows, ko, q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
+            mask.data_ptr() if mask is not None else 0, s, scale)
+    return q, k, v, args, _lib.load().pcm_cross_attn_ws_bytes(b, h, hkv, d, l, q_rows, qo != 0, s, kv_rows, ko != 0)
 
 
-def _workspace(L_, sides, dev):
-    b, h, hkv, d, l, q_rows, qo, s, kv_rows, ko = sides
-    n = L_.pcm_cross_attn_ws_bytes(b, h, hkv, d, l, q_rows, int(qo != 0), s, kv_rows, int(ko != 0))
-    return torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _operands(q, k, v, mask, scale):
-    mask_bs = mask.stride(0) if mask is not None and mask.dim() == 2 else 0
-    return (q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), _ptr(mask), mask_bs, scale)
+def _forward(q, k, v, mask, q_offset, kv_offset, scale, want_lse):
+    dev = q.device
+    with _lib.on_device(dev):
+        q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, scale)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        out = _new(q)
+        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
+        rc = _lib.load().pcm_cross_attn_forward_hip(*args, out.data_ptr(), lse.data_ptr() if want_lse else 0, ws.data_ptr() if ws_bytes else 0,
+                                                    ws_bytes, _raw_stream())
+    if rc:
+        _lib.check(rc, "pcm_cross_attn_forward_hip")
+    return out, lse, q, k, v
 
 
 class _CrossAttention(Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask, q_offset, kv_offset, scale, want_lse):
-        L_ = _lib.load()
-        q, k, v = _fit(q), _fit(k), _fit(v)
-        dev = q.device
-        grad = any(ctx.needs_input_grad[:3])
-        with torch.cuda.device(dev):
-            sides = _sides(q, k, q_offset, kv_offset)
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-            lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if grad or want_lse else None
-            ws = _workspace(L_, sides, dev)
-            rc = L_.pcm_cross_attn_forward_hip(*sides, *_operands(q, k, v, mask, scale), out.data_ptr(), _ptr(lse), _ptr(ws),
-                                               ws.numel() * 4 if ws is not None else 0, _raw_stream())
-        _lib.check(rc, "pcm_cross_attn_forward_hip")
-        if lse is not None:
-            ctx.mark_non_differentiable(lse)
-        if grad:
-            ctx.save_for_backward(q, k, v, mask, q_offset, kv_offset, out, lse)
-            ctx.scale = scale
+    def forward(ctx, q, k, v, mask, q_offset, kv_offset, scale):
+        out, lse, q, k, v = _forward(q, k, v, mask, q_offset, kv_offset, scale, True)
+        ctx.mark_non_differentiable(lse)
+        ctx.save_for_backward(q, k, v, mask, q_offset, kv_offset, out, lse)
+        ctx.scale = scale
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _):
-        L_ = _lib.load()
         q, k, v, mask, q_offset, kv_offset, out, lse = ctx.saved_tensors
-        dout = _fit(dout)
         dev = q.device
-        with torch.cuda.device(dev):
-            sides = _sides(q, k, q_offset, kv_offset)
-            dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-            dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2))
-            delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
-            ws = _workspace(L_, sides, dev)
-            rc = L_.pcm_cross_attn_backward_hip(*sides, *_operands(q, k, v, mask, ctx.scale), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                                *_strides(dout), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws),
-                                                ws.numel() * 4 if ws is not None else 0, _raw_stream())
-        _lib.check(rc, "pcm_cross_attn_backward_hip")
-        return dq, dk, dv, None, None, None, None, None
+        with _lib.on_device(dev):
+            q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale)
+            dout, gs = _fit(dout)
+            dq, dk, dv = _new(q), _new(k), _new(v)
+            at = lse.numel() * 4 + 15 & ~15
+            ws = torch.empty(at + ws_bytes, dtype=torch.uint8, device=dev)  # delta, then the workspace
+            p = ws.data_ptr()
+            rc = _lib.load().pcm_cross_attn_backward_hip(*args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), *gs, p, dq.data_ptr(),
+                                                         dk.data_ptr(), dv.data_ptr(), p + at, ws_bytes, _raw_stream())
+        if rc:
+            _lib.check(rc, "pcm_cross_attn_backward_hip")
+        return dq, dk, dv, None, None, None, None
 
 
 def _check_offset(offset, side, t, name):
@@ -137,10 +130,13 @@ def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=Non
     if mask is not None:
         if mask.dtype != torch.bool or mask.shape != k.shape[:-2] or mask.device != k.device:
             raise ValueError("cross_attention: key_padding_mask must be a bool tensor %s on %s" % (tuple(k.shape[:-2]), k.device))
-        mask = mask.contiguous().view(torch.uint8)
+        mask = mask.contiguous()
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("cross_attention: scale must be positive and finite, got %r" % (scale,))
-    out, lse = _CrossAttention.apply(q, k, v, mask, q_offset, kv_offset, scale, bool(return_lse))
-    _graphs.guard_leaves(out, "cross_attention")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _CrossAttention.apply(q, k, v, mask, q_offset, kv_offset, scale)
+        _graphs.guard_leaves(out, "cross_attention")
+    else:
+        out, lse, *_ = _forward(q, k, v, mask, q_offset, kv_offset, scale, return_lse)
     return (out, lse) if return_lse else out

@@ -10,68 +10,77 @@ from ..pointops import _common
 from .._lib import raw_stream as _raw_stream
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+_NAMES = ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
 
 
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _workspace(L_, rows, e, f, backward, dev):
-    n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, int(backward))
-    return n, (torch.empty(n, dtype=torch.uint8, device=dev) if n else None)
-
-
 def _rows(t, width):
     """(rows, width) with contiguous channels: a view where the strides allow one."""
-    t = t.reshape(-1, width)
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
     return t if t.stride(-1) == 1 or width == 1 else t.contiguous()
+
+
+def _empty(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
+    """y, and for a backward pass (keep) the hidden tensors a | u | h in one buffer, else None."""
+    L_ = _lib.load()
+    (rows, e), f, dev = x.shape, w_gate.shape[0], x.device
+    with _lib.on_device(dev):
+        ld = L_.pcm_gated_ffn_hidden_ld(f)
+        n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, False)
+        y = torch.empty((rows, e), dtype=x.dtype, device=dev)
+        size = 2 * rows * ld
+        hidden = _empty(3 * size if keep else size + n, dev)  # without a backward pass: h, then the workspace
+        p = hidden.data_ptr()
+        a, u, h = (p, p + size, p + 2 * size) if keep else (0, 0, p)
+        ws = _empty(n, dev) if keep and n else None
+        rc = L_.pcm_gated_ffn_forward_hip(rows, e, f, act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+                                          _ptr(b_gate), _ptr(b_up), _ptr(b_down), y.data_ptr(), a, u, h, _ptr(ws) if keep else p + size, n,
+                                          _raw_stream())
+    if rc:
+        _lib.check(rc, "pcm_gated_ffn_forward_hip")
+    return y, hidden if keep else None
 
 
 class _GatedFFN(Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-        L_ = _lib.load()
-        rows, e = x.shape
-        f = w_gate.shape[0]
-        w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
-        b_gate, b_up, b_down = (b.contiguous() if b is not None else None for b in (b_gate, b_up, b_down))
-        grad = any(ctx.needs_input_grad[:7])
-        with torch.cuda.device(x.device):
-            ld = L_.pcm_gated_ffn_hidden_ld(f)
-            y = torch.empty(rows, e, dtype=x.dtype, device=x.device)
-            a, u, h = torch.empty(3 if grad else 1, rows, ld, dtype=x.dtype, device=x.device) if grad else (None, None, torch.empty(rows, ld, dtype=x.dtype, device=x.device))
-            n, ws = _workspace(L_, rows, e, f, False, x.device)
-            rc = L_.pcm_gated_ffn_forward_hip(rows, e, f, act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-                                              _ptr(b_gate), _ptr(b_up), _ptr(b_down), y.data_ptr(), _ptr(a), _ptr(u), h.data_ptr(),
-                                              _ptr(ws), n, _raw_stream())
-        _lib.check(rc, "pcm_gated_ffn_forward_hip")
-        if grad:
-            ctx.save_for_backward(x, w_gate, w_up, w_down, a, u, h)
-            ctx.act = act
+        y, hidden = _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, hidden)
+        ctx.act = act
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         L_ = _lib.load()
-        x, w_gate, w_up, w_down, a, u, h = ctx.saved_tensors
+        x, w_gate, w_up, w_down, hidden = ctx.saved_tensors
         need = ctx.needs_input_grad
-        (rows, e), f, dev = x.shape, w_gate.shape[0], x.device
+        (rows, e), f, dev, dtype = x.shape, w_gate.shape[0], x.device, x.dtype
         dy = _rows(dy, e)
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             new = torch.zeros if rows == 0 else torch.empty  # no rows: no launch, the gradients of the weights are zero
-            dx = new(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-            dwg, dwu = (new(f, e, dtype=x.dtype, device=dev) if need[1] or need[2] else None for _ in range(2))
-            dwd = new(e, f, dtype=x.dtype, device=dev) if need[3] else None
-            dbg, dbu = (new(f, dtype=x.dtype, device=dev) if need[4] or need[5] else None for _ in range(2))
-            dbd = new(e, dtype=x.dtype, device=dev) if need[6] else None
-            n, ws = _workspace(L_, rows, e, f, True, dev)
+            dx = new((rows, e), dtype=dtype, device=dev) if need[0] else None
+            dwg, dwu = new((2, f, e), dtype=dtype, device=dev).unbind() if need[1] or need[2] else (None, None)
+            dwd = new((e, f), dtype=dtype, device=dev) if need[3] else None
+            dbg, dbu = new((2, f), dtype=dtype, device=dev).unbind() if need[4] or need[5] else (None, None)
+            dbd = new((e,), dtype=dtype, device=dev) if need[6] else None
+            n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, True)
+            ws = _empty(n, dev)
+            p, size = hidden.data_ptr(), hidden.numel() // 3
             rc = L_.pcm_gated_ffn_backward_hip(rows, e, f, ctx.act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
-                                               w_down.data_ptr(), a.data_ptr(), u.data_ptr(), h.data_ptr(), dy.data_ptr(), dy.stride(0),
-                                               _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), _ptr(ws), n,
-                                               _raw_stream())
-        _lib.check(rc, "pcm_gated_ffn_backward_hip")
-        return (dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dbg if need[4] else None, dbu if need[5] else None, dbd, None)
+                                               w_down.data_ptr(), p, p + size, p + 2 * size, dy.data_ptr(), dy.stride(0), _ptr(dx), _ptr(dwg),
+                                               _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), ws.data_ptr(), n, _raw_stream())
+        if rc:
+            _lib.check(rc, "pcm_gated_ffn_backward_hip")
+        return dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dbg if need[4] else None, dbu if need[5] else None, dbd, None
 
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation="silu"):
@@ -83,23 +92,28 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     _common.require_hip(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     if activation not in ACTIVATIONS:
         raise ValueError("gated_ffn: activation should be silu/gelu/relu, not %r" % (activation,))
-    given = [x, w_gate, w_up, w_down, b_gate, b_up, b_down]
+    given = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
-        given = [t.to(torch.bfloat16) if t is not None and t.is_floating_point() else t for t in given]
-    for t, name in zip(given, ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")):
-        if t is not None and t.dtype != torch.bfloat16:
-            raise TypeError("gated_ffn: %s must be bfloat16 (or the call under bf16 autocast), got %s" % (name, t.dtype))
-        if t is not None and t.device != x.device:
+        given = tuple(t.to(torch.bfloat16) if t is not None and t.is_floating_point() else t for t in given)
+    for t, name in zip(given, _NAMES):
+        if t is not None and (t.dtype is not torch.bfloat16 or t.device != x.device):
+            if t.dtype is not torch.bfloat16:
+                raise TypeError("gated_ffn: %s must be bfloat16 (or the call under bf16 autocast), got %s" % (name, t.dtype))
             raise ValueError("gated_ffn: x is on %s, %s on %s" % (x.device, name, t.device))
     x, w_gate, w_up, w_down, b_gate, b_up, b_down = given
-    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or min(w_gate.shape) < 1:
-        raise ValueError("gated_ffn: shapes x %s, w_gate %s, w_up %s" % (tuple(x.shape), tuple(w_gate.shape), tuple(w_up.shape)))
-    f, e = w_gate.shape
-    if x.shape[-1] != e or tuple(w_down.shape) != (e, f):
-        raise ValueError("gated_ffn: x %s, w_gate %s, w_down %s" % (tuple(x.shape), (f, e), tuple(w_down.shape)))
+    shape, ws = x.shape, w_gate.shape
+    if len(shape) < 1 or len(ws) != 2 or ws != w_up.shape or min(ws) < 1:
+        raise ValueError("gated_ffn: shapes x %s, w_gate %s, w_up %s" % (tuple(shape), tuple(ws), tuple(w_up.shape)))
+    f, e = ws
+    if shape[-1] != e or w_down.shape != (e, f):
+        raise ValueError("gated_ffn: x %s, w_gate %s, w_down %s" % (tuple(shape), (f, e), tuple(w_down.shape)))
     for b, n, name in ((b_gate, f, "b_gate"), (b_up, f, "b_up"), (b_down, e, "b_down")):
-        if b is not None and tuple(b.shape) != (n,):
+        if b is not None and b.shape != (n,):
             raise ValueError("gated_ffn: %s must be (%d,), got %s" % (name, n, tuple(b.shape)))
-    rows = _rows(x, e)
-    y = _GatedFFN.apply(rows, w_gate, w_up, w_down, b_gate, b_up, b_down, ACTIVATIONS[activation])
-    return _graphs.guard_leaves(y, "gated_ffn").view(x.shape)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given)
+    args = [_rows(x, e)] + [t if t is None or t.is_contiguous() else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    if grad:
+        y = _graphs.guard_leaves(_GatedFFN.apply(*args, ACTIVATIONS[activation]), "gated_ffn")
+    else:
+        y, _ = _forward(*args, ACTIVATIONS[activation], False)
+    return y if len(shape) == 2 else y.view(shape)
