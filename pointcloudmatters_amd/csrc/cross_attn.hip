@@ -93,15 +93,6 @@ __device__ __forceinline__ long xa_item(long items)
 typedef s4 __attribute__((address_space(3))) * xa_lds_s4;
 __device__ __forceinline__ s4 xa_tr(const u16 *p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((xa_lds_s4)p); }
 
-// Transposed operand: lane <-> channel 32 * blk + lane % 32, contracted index i of half h <-> tile row row16 + 4 h + i % 4 + 8 (i / 4):
-// the order in which a 32 x 32 accumulator holds 16 of its rows.
-template <int LD>
-__device__ __forceinline__ bf8 xa_transposed(const u16 *tile, int row16, int blk, int lane)
-{
-    const int p = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
-    const u16 *a = tile + (row16 + 4 * h + (p >> 2)) * LD + 32 * blk + 16 * g + 4 * (p & 3);
-    return cat8(xa_tr(a), xa_tr(a + 8 * LD));
-}
 __device__ __forceinline__ f16v xa_zero16()
 {
     f16v z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -121,53 +112,106 @@ __device__ __forceinline__ void xa_row_operand(const u16 *row, bool ok, int D, i
         f[t] = as_bf8(ok && 16 * t + 8 * h < D ? *(const uint4 *)(row + 16 * t + 8 * h) : make_uint4(0, 0, 0, 0));
 }
 
-// 64 rows of a strided matrix on their way into LDS: 16-byte pieces, DP / 32 per thread, requested together.
-template <int DP>
-struct XaStage {
-    static constexpr int N = DP / 32, PIECES = DP / 8, LD = DP + 8;
-    uint4 d[N];
-    __device__ __forceinline__ void load(const u16 *base, long ls, int row0, int n, int D)
-    {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = threadIdx.x + 256 * i, r = c / PIECES, p = c - r * PIECES;
-            d[i] = row0 + r < n && 8 * p < D ? *(const uint4 *)(base + (long)(row0 + r) * ls + 8 * p) : make_uint4(0, 0, 0, 0);
-        }
-    }
-    // visible: bit r <-> row r of the tile
-    __device__ __forceinline__ void store(u16 *tile, unsigned long long visible) const
-    {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = threadIdx.x + 256 * i, r = c / PIECES, p = c - r * PIECES;
-            const bool keep = (visible >> r) & 1;
-            *(uint4 *)(tile + r * LD + 8 * p) = keep ? d[i] : make_uint4(0, 0, 0, 0);
-        }
-    }
-};
+// Tiles of 64 rows x DP channels in LDS, filled by global_load_lds: a wave's 64 16-byte pieces go to consecutive addresses, no registers
+// and no LDS write instructions.  That layout cannot be padded, so the piece a slot holds is permuted by its row (the lane picks its
+// source): the 8 lanes that read one piece of 8 neighbouring rows, and the 4 rows x 2 pieces of a 16-lane group of ds_read_b64_tr_b16, meet
+// different banks.  Pieces outside (absent or masked rows, channels from D on) are read from a block of zeros.
+__device__ uint4 xa_zeros;
+typedef __attribute__((address_space(3))) void *xa_lds_p;
+typedef const __attribute__((address_space(1))) void *xa_glb_p;
 
-// rows r = token * G + g of a strided (token, head, channel) matrix
 template <int DP>
-struct XaRowStage {
-    static constexpr int N = DP / 32, PIECES = DP / 8, LD = DP + 8;
-    uint4 d[N];
-    __device__ __forceinline__ void load(const u16 *base, long ls, long hs, int row0, int n, int G, int D)
+__device__ __forceinline__ int xa_swz(int r)
+{
+    if constexpr (DP >= 64) return ((r & 3) << 1) | ((r >> 2) & 1);
+    else return (((r >> 1) & 1) << 1) | ((r >> 2) & 1);  // two rows in 128 bytes
+}
+template <int DP>
+__device__ __forceinline__ int xa_at(int row, int piece)  // value offset of a piece inside a tile
+{
+    return row * DP + ((piece ^ xa_swz<DP>(row)) << 3);
+}
+
+// THREADS threads (a workgroup or one wave) request ROWS rows; a thread's n-th piece stands n * NR rows below its first.
+template <int DP, int ROWS, int THREADS>
+struct XaStage {
+    static constexpr int PIECES = DP / 8, NR = THREADS / PIECES, N = ROWS / NR;
+    int r;        // tile row of the first piece
+    int p;        // its channel
+    bool in;      // p < D
+    int dim;
+    static_assert(NR % 8 == 0 || (NR == 4 && DP >= 64), "see load()");
+    __device__ __forceinline__ void init(int t, int D)
     {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = threadIdx.x + 256 * i, r = c / PIECES, p = c - r * PIECES, row = row0 + r, tok = row / G;
-            d[i] = row < n && 8 * p < D ? *(const uint4 *)(base + (long)tok * ls + (long)(row - tok * G) * hs + 8 * p) : make_uint4(0, 0, 0, 0);
-        }
+        r = t / PIECES, p = 8 * ((t - r * PIECES) ^ xa_swz<DP>(r)), in = p < D, dim = D;
     }
-    __device__ __forceinline__ void store(u16 *tile) const
+    static __device__ __forceinline__ void put(const u16 *src, bool ok, u16 *tile, int n, int wave)
     {
+        __builtin_amdgcn_global_load_lds((xa_glb_p)(ok ? (const void *)src : (const void *)&xa_zeros), (xa_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, 0, 0);
+    }
+    // rows row0 .. of a matrix at row stride ls; visible: bit i <-> tile row i
+    __device__ __forceinline__ void load(const u16 *base, long ls, long row0, unsigned long long visible, u16 *tile, int wave) const
+    {
+        const u16 *src = base + (row0 + r) * ls;
+        const unsigned long long mine = visible >> r;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = threadIdx.x + 256 * i, r = c / PIECES, p = c - r * PIECES;
-            *(uint4 *)(tile + r * LD + 8 * p) = d[i];
+        for (int n = 0; n < N; ++n) {
+            // the permutation repeats every 8 rows; 4 rows further it is its neighbour's
+            const int pn = NR % 8 != 0 && (n & 1) ? p ^ 8 : p;
+            put(src + n * (NR * ls) + pn, (NR % 8 != 0 ? pn < dim : in) && ((mine >> (n * NR)) & 1), tile, n, wave);
         }
     }
 };
+// rows = token * G + g of a (token, head, channel) matrix
+template <int DP, int ROWS>
+struct XaRowStage : XaStage<DP, ROWS, 256> {
+    typedef XaStage<DP, ROWS, 256> Base;
+    __device__ __forceinline__ void load_rows(const u16 *a, long a_ls, long a_hs, u16 *ta, const u16 *b, long b_ls, long b_hs, u16 *tb, int row0, int n, int G, int wave) const
+    {
+#pragma unroll
+        for (int i = 0; i < Base::N; ++i) {
+            const int row = row0 + Base::r + i * Base::NR, tok = G == 1 ? row : row / G, g = row - tok * G;
+            const bool ok = Base::in && row < n;
+            Base::put(a + tok * a_ls + g * a_hs + Base::p, ok, ta, i, wave);
+            Base::put(b + tok * b_ls + g * b_hs + Base::p, ok, tb, i, wave);
+        }
+    }
+};
+// all of this wave's requests have arrived and its LDS reads are done; then the same of every wave
+__device__ __forceinline__ void xa_arrived()
+{
+    __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0)
+    __syncthreads();
+}
+// which of the 64 (or fewer) keys from key0 on are there and seen: bit i <-> key0 + i
+__device__ __forceinline__ unsigned long long xa_visible(const unsigned char *mask, unsigned byte, int key0, int n, int lane)
+{
+    if (mask != nullptr) return __ballot(key0 + lane < n && byte == 0u);
+    const int left = n - key0;
+    return left >= 64 ? ~0ull : (left <= 0 ? 0ull : (1ull << left) - 1);
+}
+// scores of keys that are not to be seen
+__device__ __forceinline__ void xa_hide(f16v &s, unsigned keys, int h, float v)
+{
+    const unsigned mine = keys >> (4 * h);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (!((mine >> ((r & 3) + 8 * (r >> 2))) & 1)) s[r] = v;
+}
+
+// Transposed operand: lane <-> channel 32 * blk + lane % 32, contracted index i of half h <-> tile row row16 + 4 h + i % 4 + 8 (i / 4):
+// the order in which a 32 x 32 accumulator holds 16 of its rows.
+template <int DP>
+__device__ __forceinline__ bf8 xa_transposed(const u16 *tile, int row16, int blk, int lane)
+{
+    const int p = lane & 15, g = (lane >> 4) & 1, h = lane >> 5, r = row16 + 4 * h + (p >> 2), c = 4 * blk + 2 * g + ((p >> 1) & 1);
+    return cat8(xa_tr(tile + xa_at<DP>(r, c) + 4 * (p & 1)), xa_tr(tile + xa_at<DP>(r + 8, c) + 4 * (p & 1)));
+}
+template <int DP>
+__device__ __forceinline__ bf8 xa_rows_operand(const u16 *tile, int row0, int t, int lane)  // lane <-> row, channels 16 t + 8 h ..
+{
+    return lds_bf8(tile + xa_at<DP>(row0 + (lane & 31), 2 * t + (lane >> 5)));
+}
 
 __device__ __forceinline__ unsigned xa_mask_byte(const unsigned char *m, int key, int n) { return m != nullptr && key < n ? (unsigned)m[key] : 0u; }
 
@@ -225,78 +269,69 @@ __device__ __forceinline__ const u16 *xa_q_row(const XaParams &P, const u16 *bas
     return base + (P.q_off ? (R.qs.row0 + R.tok) * ls : R.b * bs + R.tok * ls) + (long)R.head * hs;
 }
 
+// One 32-row column of the forward pass: running maximum m and sum l (of this lane's half of the keys) and O^T.
 template <int DP>
-__global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
-{
-    constexpr int LD = DP + 8;
-    __shared__ __attribute__((aligned(16))) u16 sk[XA_TILE * LD], sv[XA_TILE * LD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-    XaRows R;
-    if (!xa_rows(P, lane, wave, R)) return;
-    bf8 qf[DP / 16];
-    xa_row_operand<DP>(xa_q_row(P, P.q, P.q_bs, P.q_ls, P.q_hs, R), R.ok, P.D, h, qf);
+struct XaSoftmax {
     f16v o[DP / 32];
+    float m, l;
+    __device__ __forceinline__ void init()
+    {
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) o[i] = xa_zero16();
-    float m = -INFINITY, l = 0.f;
-    const float c = P.scale * XA_LOG2E;
-    XaStage<DP> gk, gv;
-    unsigned mb = 0;
-    if (R.key_lo < R.key_hi) {
-        mb = xa_mask_byte(R.mask, R.key_lo + lane, R.ks.n);
-        gk.load(R.k, P.k_ls, R.key_lo, R.ks.n, P.D), gv.load(R.v, P.v_ls, R.key_lo, R.ks.n, P.D);
+        for (int i = 0; i < DP / 32; ++i) o[i] = xa_zero16();
+        m = -INFINITY, l = 0.f;
     }
-    for (int key0 = R.key_lo; key0 < R.key_hi; key0 += XA_TILE) {
-        const unsigned long long vis = __ballot(key0 + lane < R.ks.n && mb == 0u);
-        __syncthreads();
-        gk.store(sk, vis), gv.store(sv, vis);
-        __syncthreads();
-        if (key0 + XA_TILE < R.key_hi) {
-            mb = xa_mask_byte(R.mask, key0 + XA_TILE + lane, R.ks.n);
-            gk.load(R.k, P.k_ls, key0 + XA_TILE, R.ks.n, P.D), gv.load(R.v, P.v_ls, key0 + XA_TILE, R.ks.n, P.D);
-        }
-        if (vis == 0) continue;
-        f16v s[2];
+    // NJ * 32 keys of a tile, c = scale * log2 e
+    template <int NJ>
+    __device__ __forceinline__ void tile(const u16 *sk, const u16 *sv, const bf8 (&qf)[DP / 16], unsigned long long vis, float c, int lane)
+    {
+        const int h = lane >> 5;
+        f16v s[NJ];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NJ; ++j) {
             s[j] = xa_zero16();
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) s[j] = PCM_MFMA16(lds_bf8(sk + (32 * j + col) * LD + 16 * t + 8 * h), qf[t], s[j]);
+            for (int t = 0; t < DP / 16; ++t) s[j] = PCM_MFMA16(xa_rows_operand<DP>(sk, 32 * j, t, lane), qf[t], s[j]);
         }
-        if (vis != ~0ull) {
-            const unsigned long long mine = vis >> (4 * h);
+        if (vis != (NJ == 2 ? ~0ull : 0xFFFFFFFFull)) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[j][r] = -INFINITY;
+            for (int j = 0; j < NJ; ++j) xa_hide(s[j], (unsigned)(vis >> (32 * j)), h, -INFINITY);
         }
         float mx = m;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = max3f(mx, s[0][r], s[1][r]);
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) mx = max3f(mx, s[j][r], s[j][r + 1]);
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float mc = mx == -INFINITY ? 0.f : mx * c;
-        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, c, -mc));
+        if (__ballot(mx > m) != 0) {  // a row's maximum has grown: after the first tiles a rare case
+            const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, c, -mc));
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+        }
         m = mx;
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -mc));
                 sum += s[j][r];
             }
-        l = __builtin_fmaf(l, alpha, sum);
+        l += sum;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 2 * NJ; ++t) {
             const bf8 p = xa_pack(s[t >> 1], t & 1);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(xa_transposed<LD>(sv, 16 * t, i, lane), p, o[i]);
+            for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(xa_transposed<DP>(sv, 16 * t, i, lane), p, o[i]);
         }
     }
-    l += __shfl_xor(l, 32);
+};
+
+// the end of a row: its result, or its part of a split
+template <int DP>
+__device__ __forceinline__ void xa_finish(const XaParams &P, const XaRows &R, const f16v (&o)[DP / 32], float m, float l, int h)
+{
     if (!R.ok) return;
     if (P.nsplit > 1) {
         const long at = (long)R.split * P.q_rows * P.H + R.out_row;
@@ -311,110 +346,215 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
     for (int i = 0; i < DP / 32; ++i) xa_store_row(P.out + R.out_row * P.D, P.D, h, i, o[i], inv);
 }
 
-// joins the splits of a row: one wave per (row, head), lanes over channels
-__global__ void __launch_bounds__(256) pcm_xattn_join_kernel(XaParams P)
+// The keys of a row kernel, 64 at a time through two LDS buffers of K and V: while tile t is worked on, tile t + 1 is on its way.  The
+// buffers are variables of their own, so that the compiler can tell reads of one from requests into the other.
+template <int DP, class F>
+__device__ __forceinline__ void xa_key_loop(const XaRows &R, const XaParams &P, u16 *sk0, u16 *sv0, u16 *sk1, u16 *sv1, int lane, int wave, F body)
 {
-    const long rows = P.q_rows * P.H, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
-    float m = -INFINITY;
-    for (int s = 0; s < P.nsplit; ++s) m = fmaxf(m, P.part_ml[2 * (s * rows + row)]);
-    const float c = P.scale * XA_LOG2E;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < P.nsplit; ++s) {
-        const float2 ml = *(const float2 *)(P.part_ml + 2 * (s * rows + row));
-        if (ml.y == 0.f) continue;  // no key in this split
-        const float w = __builtin_amdgcn_exp2f((ml.x - m) * c);
-        l = __builtin_fmaf(ml.y, w, l);
-        const float *po = P.part_o + (s * rows + row) * P.D;
-        if (2 * lane < P.D) o0 = __builtin_fmaf(po[2 * lane], w, o0), o1 = __builtin_fmaf(po[2 * lane + 1], w, o1);
+    if (R.key_lo >= R.key_hi) return;
+    XaStage<DP, XA_TILE, 256> st;
+    st.init((int)threadIdx.x, P.D);
+    unsigned mb = xa_mask_byte(R.mask, R.key_lo + lane, R.ks.n);
+    unsigned long long next = 0;
+    const auto request = [&](int key0, u16 *tk, u16 *tv) {
+        next = xa_visible(R.mask, mb, key0, R.ks.n, lane);
+        st.load(R.k, P.k_ls, key0, next, tk, wave), st.load(R.v, P.v_ls, key0, next, tv, wave);
+        mb = xa_mask_byte(R.mask, key0 + XA_TILE + lane, R.ks.n);
+    };
+    const auto step = [&](int key0, const u16 *tk, const u16 *tv, u16 *nk, u16 *nv) {
+        xa_arrived();
+        const unsigned long long vis = next;
+        if (key0 + XA_TILE < R.key_hi) request(key0 + XA_TILE, nk, nv);
+        if (vis != 0) body(tk, tv, vis);
+    };
+    request(R.key_lo, sk0, sv0);
+    int key0 = R.key_lo;
+    for (; key0 + XA_TILE < R.key_hi; key0 += 2 * XA_TILE) {
+        step(key0, sk0, sv0, sk1, sv1);
+        step(key0 + XA_TILE, sk1, sv1, sk0, sv0);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (P.lse && lane == 0) P.lse[row] = l == 0.f ? -INFINITY : m * P.scale + __logf(l);
-    if (2 * lane < P.D) *(uint32_t *)(P.out + row * P.D + 2 * lane) = cvt_pk_bf16(o0 * inv, o1 * inv);
-}
-
-// delta = rowsum(dO * O): 16 lanes per (row, head), 8 channels each
-__global__ void __launch_bounds__(256) pcm_xattn_delta_kernel(XaParams P)
-{
-    const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int d = 8 * (threadIdx.x & 15);
-    float s = 0.f;
-    if (row < P.q_rows * P.H && d < P.D) {
-        const long tok = row / P.H, head = row - tok * P.H;
-        const long b = P.q_off ? 0 : tok / P.L, l = P.q_off ? tok : tok - b * P.L;
-        const uint4 a = *(const uint4 *)(P.out + row * P.D + d), g = *(const uint4 *)(P.dout + b * P.g_bs + l * P.g_ls + head * P.g_hs + d);
-        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s = __builtin_fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
-            s = __builtin_fmaf(__uint_as_float(x[i] & 0xFFFF0000u), __uint_as_float(y[i] & 0xFFFF0000u), s);
-        }
-    }
-    for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k);
-    if ((threadIdx.x & 15) == 0 && row < P.q_rows * P.H) P.delta[row] = s;
+    if (key0 < R.key_hi) step(key0, sk0, sv0, sk1, sv1);
 }
 
 template <int DP>
+__global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
+{
+    __shared__ __attribute__((aligned(1024))) u16 sk0[XA_TILE * DP], sv0[XA_TILE * DP], sk1[XA_TILE * DP], sv1[XA_TILE * DP];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
+    XaRows R;
+    if (!xa_rows(P, lane, wave, R)) return;
+    bf8 qf[DP / 16];
+    xa_row_operand<DP>(xa_q_row(P, P.q, P.q_bs, P.q_ls, P.q_hs, R), R.ok, P.D, h, qf);
+    XaSoftmax<DP> w;
+    w.init();
+    const float c = P.scale * XA_LOG2E;
+    xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, lane, wave,
+                    [&](const u16 *tk, const u16 *tv, unsigned long long vis) { w.template tile<2>(tk, tv, qf, vis, c, lane); });
+    w.l += __shfl_xor(w.l, 32);
+    xa_finish<DP>(P, R, w.o, w.m, w.l, h);
+}
+
+// Few rows (up to 32 of a key head: one token of a rollout, a group of heads that share one): all four waves hold the same rows and share
+// the keys, wave w every fourth run of 32, each with LDS tiles and waits of its own (no barrier until the end).  K and V are read once and
+// nothing else is long, so what counts is requests in flight: two tiles of K and V a wave.  The waves' sums are joined through LDS.
+template <int DP>
+__global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
+{
+    constexpr int TILE = 32 * DP;
+    __shared__ __attribute__((aligned(1024))) u16 t0[4 * 2 * TILE], t1[4 * 2 * TILE];
+    __shared__ float sm[4][32], sl[4][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+    XaRows R;
+    if (!xa_rows(P, lane, 0, R)) return;
+    bf8 qf[DP / 16];
+    xa_row_operand<DP>(xa_q_row(P, P.q, P.q_bs, P.q_ls, P.q_hs, R), R.ok, P.D, h, qf);
+    XaSoftmax<DP> w;
+    w.init();
+    const float c = P.scale * XA_LOG2E;
+    XaStage<DP, 32, 64> st;
+    st.init(lane, P.D);
+    u16 *const k0 = t0 + wave * 2 * TILE, *const k1 = t1 + wave * 2 * TILE;
+    unsigned mb = 0;
+    unsigned long long vis = 0, next = 0;
+    const auto request = [&](int key0, u16 *tk) {
+        next = xa_visible(R.mask, mb, key0, R.ks.n, lane) & 0xFFFFFFFFull;
+        st.load(R.k, P.k_ls, key0, next, tk, 0), st.load(R.v, P.v_ls, key0, next, tk + TILE, 0);
+        mb = xa_mask_byte(R.mask, key0 + 128 + lane, R.ks.n);
+    };
+    const auto step = [&](int key0, const u16 *tk, u16 *nk) {
+        __builtin_amdgcn_s_waitcnt(0x70);  // this wave's tile has arrived, its reads of the other are done
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        vis = next;
+        if (key0 + 128 < R.key_hi) request(key0 + 128, nk);
+        if (vis != 0) w.template tile<1>(tk, tk + TILE, qf, vis, c, lane);
+    };
+    int key0 = R.key_lo + 32 * wave;
+    if (key0 < R.key_hi) {
+        mb = xa_mask_byte(R.mask, key0 + lane, R.ks.n);
+        request(key0, k0);
+        for (; key0 + 128 < R.key_hi; key0 += 256) {
+            step(key0, k0, k1);
+            step(key0 + 128, k1, k0);
+        }
+        if (key0 < R.key_hi) step(key0, k0, k1);
+    }
+    w.l += __shfl_xor(w.l, 32);
+    if (h == 0) sm[wave][col] = w.m, sl[wave][col] = w.l;
+    __syncthreads();
+    float m = sm[0][col];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = fmaxf(m, sm[i][col]);
+    float l = 0.f, mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = sl[i][col] == 0.f ? 0.f : __builtin_amdgcn_exp2f((sm[i][col] - m) * c);
+        if (sl[i][col] != 0.f) l = __builtin_fmaf(sl[i][col], f, l);
+        if (i == wave) mine = f;
+    }
+    // O^T of the waves, one after the other in wave order: [register][lane] in the tiles' memory (4 * DP * 2 bytes a lane fit)
+    float *const sum = (float *)t0;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float v = mine == 0.f && w.l == 0.f ? 0.f : w.o[i][r] * mine;
+            if (wave != 0) sum[((wave - 1) * (DP / 2) + 16 * i + r) * 64 + lane] = v;
+            else w.o[i][r] = v;
+        }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) w.o[i][r] += sum[(k * (DP / 2) + 16 * i + r) * 64 + lane];
+    xa_finish<DP>(P, R, w.o, m, l, h);
+}
+
+// joins the splits of a row in split order: LPR lanes per (row, head), four channels each
+template <int LPR>
+__global__ void __launch_bounds__(256) pcm_xattn_join_kernel(XaParams P)
+{
+    const long rows = P.q_rows * P.H, row = (long)blockIdx.x * (256 / LPR) + (int)threadIdx.x / LPR;
+    const int d = 4 * ((int)threadIdx.x % LPR);
+    if (row >= rows) return;
+    const float2 *ml = (const float2 *)P.part_ml + row;
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < P.nsplit; ++s) m = fmaxf(m, ml[s * rows].x);
+    const float c = P.scale * XA_LOG2E;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < P.D) {
+#pragma unroll 4
+        for (int s = 0; s < P.nsplit; ++s) {
+            const float2 w = ml[s * rows];
+            const float4 v = *(const float4 *)(P.part_o + (s * rows + row) * P.D + d);
+            if (w.y != 0.f) {  // a split without a key holds no sum
+                const float f = __builtin_amdgcn_exp2f((w.x - m) * c);
+                l = __builtin_fmaf(w.y, f, l);
+                o.x = __builtin_fmaf(v.x, f, o.x), o.y = __builtin_fmaf(v.y, f, o.y), o.z = __builtin_fmaf(v.z, f, o.z), o.w = __builtin_fmaf(v.w, f, o.w);
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (P.lse && d == 0) P.lse[row] = l == 0.f ? -INFINITY : m * P.scale + __logf(l);
+        *(uint2 *)(P.out + row * P.D + d) = make_uint2(cvt_pk_bf16(o.x * inv, o.y * inv), cvt_pk_bf16(o.z * inv, o.w * inv));
+    }
+}
+
+// dQ, and delta = rowsum(dO * O) on the way (the key kernel, launched behind, reads it)
+template <int DP>
 __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
 {
-    constexpr int LD = DP + 8;
-    __shared__ __attribute__((aligned(16))) u16 sk[XA_TILE * LD], sv[XA_TILE * LD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    __shared__ __attribute__((aligned(1024))) u16 sk0[XA_TILE * DP], sv0[XA_TILE * DP], sk1[XA_TILE * DP], sv1[XA_TILE * DP];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
     XaRows R;
     if (!xa_rows(P, lane, wave, R)) return;
     bf8 qf[DP / 16], gf[DP / 16];
+    float delta = 0.f;
+    {
+        bf8 of[DP / 16];
+        xa_row_operand<DP>(P.out + R.out_row * P.D, R.ok, P.D, h, of);
+        xa_row_operand<DP>(xa_q_row(P, P.dout, P.g_bs, P.g_ls, P.g_hs, R), R.ok, P.D, h, gf);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)of[t][e], (float)gf[t][e], delta);
+        delta += __shfl_xor(delta, 32);
+    }
     xa_row_operand<DP>(xa_q_row(P, P.q, P.q_bs, P.q_ls, P.q_hs, R), R.ok, P.D, h, qf);
-    xa_row_operand<DP>(xa_q_row(P, P.dout, P.g_bs, P.g_ls, P.g_hs, R), R.ok, P.D, h, gf);
-    const float lse = R.ok ? P.lse[R.out_row] : -INFINITY, delta = R.ok ? P.delta[R.out_row] : 0.f;
+    if (R.ok && h == 0 && R.split == 0) P.delta[R.out_row] = delta;
+    const float lse = R.ok ? P.lse[R.out_row] : -INFINITY;
     const float l2 = lse == -INFINITY ? INFINITY : lse * XA_LOG2E;  // a row without a key: every weight 2^-inf = 0
     const float c = P.scale * XA_LOG2E;
     f16v o[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = xa_zero16();
-    XaStage<DP> gk, gv;
-    unsigned mb = 0;
-    if (R.key_lo < R.key_hi) {
-        mb = xa_mask_byte(R.mask, R.key_lo + lane, R.ks.n);
-        gk.load(R.k, P.k_ls, R.key_lo, R.ks.n, P.D), gv.load(R.v, P.v_ls, R.key_lo, R.ks.n, P.D);
-    }
-    for (int key0 = R.key_lo; key0 < R.key_hi; key0 += XA_TILE) {
-        const unsigned long long vis = __ballot(key0 + lane < R.ks.n && mb == 0u);
-        __syncthreads();
-        gk.store(sk, vis), gv.store(sv, vis);
-        __syncthreads();
-        if (key0 + XA_TILE < R.key_hi) {
-            mb = xa_mask_byte(R.mask, key0 + XA_TILE + lane, R.ks.n);
-            gk.load(R.k, P.k_ls, key0 + XA_TILE, R.ks.n, P.D), gv.load(R.v, P.v_ls, key0 + XA_TILE, R.ks.n, P.D);
-        }
-        if (vis == 0) continue;
-        const unsigned long long mine = vis >> (4 * h);
+    xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, lane, wave, [&](const u16 *tk, const u16 *tv, unsigned long long vis) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             f16v s = xa_zero16(), dp = xa_zero16();
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
-                s = PCM_MFMA16(lds_bf8(sk + (32 * j + col) * LD + 16 * t + 8 * h), qf[t], s);
-                dp = PCM_MFMA16(lds_bf8(sv + (32 * j + col) * LD + 16 * t + 8 * h), gf[t], dp);
+                s = PCM_MFMA16(xa_rows_operand<DP>(tk, 32 * j, t, lane), qf[t], s);
+                dp = PCM_MFMA16(xa_rows_operand<DP>(tv, 32 * j, t, lane), gf[t], dp);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -l2));
                 s[r] = p * (dp[r] - delta);
             }
-            if (vis != ~0ull) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[r] = 0.f;
-            }
+            if (vis != ~0ull) xa_hide(s, (unsigned)(vis >> (32 * j)), h, 0.f);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const bf8 ds = xa_pack(s, u);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(xa_transposed<LD>(sk, 32 * j + 16 * u, i, lane), ds, o[i]);
+                for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(xa_transposed<DP>(tk, 32 * j + 16 * u, i, lane), ds, o[i]);
             }
         }
-    }
+    });
     if (!R.ok) return;
     const long at = (long)R.split * P.q_rows * P.H + R.out_row;
 #pragma unroll
@@ -424,26 +564,26 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
     }
 }
 
-// dQ of a row out of its splits, in split order
+// dQ of a row out of its splits, in split order: four channels a thread (D is a multiple of 8)
 __global__ void __launch_bounds__(256) pcm_xattn_dq_join_kernel(XaParams P)
 {
-    const long pairs = P.q_rows * P.H * (P.D / 2), i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= pairs) return;
-    float a = 0.f, b = 0.f;
+    const long quads = P.q_rows * P.H * (P.D / 4), i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads) return;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int s = 0; s < P.nsplit; ++s) {
-        const float2 v = *(const float2 *)(P.part_o + 2 * (s * pairs + i));
-        a += v.x, b += v.y;
+        const float4 v = *(const float4 *)(P.part_o + 4 * (s * quads + i));
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
     }
-    *(uint32_t *)(P.dq + 2 * i) = cvt_pk_bf16(a * P.scale, b * P.scale);
+    *(uint2 *)(P.dq + 4 * i) = make_uint2(cvt_pk_bf16(a.x * P.scale, a.y * P.scale), cvt_pk_bf16(a.z * P.scale, a.w * P.scale));
 }
 
 template <int DP>
 __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) pcm_xattn_dkv_kernel(XaParams P)
 {
-    constexpr int LD = DP + 8;
-    __shared__ __attribute__((aligned(16))) u16 sq[XA_TILE * LD], sg[XA_TILE * LD];
-    __shared__ __attribute__((aligned(16))) float sl[XA_TILE], sd[XA_TILE];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    __shared__ __attribute__((aligned(1024))) u16 sq0[XA_TILE * DP], sg0[XA_TILE * DP], sq1[XA_TILE * DP], sg1[XA_TILE * DP];
+    __shared__ __attribute__((aligned(16))) float sl[2][XA_TILE], sd[2][XA_TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     const long items = (long)P.tiles * P.Hkv, item = xa_item(items);
     if (item >= items) return;
     int b, tile;
@@ -464,36 +604,34 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) pcm_xattn_dkv_kernel(XaP
     f16v dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = xa_zero16(), dv[i] = xa_zero16();
-    XaRowStage<DP> rq, rg;
-    float rl = INFINITY, rd = 0.f;
-    const auto stats = [&](int row0) {  // thread t < 64: row row0 + t
+    XaRowStage<DP, XA_TILE> st;
+    st.init((int)threadIdx.x, P.D);
+    float rl = -INFINITY, rd = 0.f;
+    const auto request = [&](int row0, u16 *tq, u16 *tg) {
+        // the statistics first, untouched until they are stored: waiting for them then leaves the tiles behind them in flight
         const int row = row0 + (int)threadIdx.x, tok = row / P.G;
-        rl = INFINITY, rd = 0.f;
+        rl = -INFINITY, rd = 0.f;
         if (threadIdx.x < XA_TILE && row < nrows) {
             const long at = (qs.row0 + tok) * P.H + kvh * P.G + (row - tok * P.G);
-            const float lse = P.lse[at];
-            rl = lse == -INFINITY ? INFINITY : lse * XA_LOG2E, rd = P.delta[at];
+            rl = P.lse[at], rd = P.delta[at];
         }
+        st.load_rows(qb, P.q_ls, P.q_hs, tq, gb, P.g_ls, P.g_hs, tg, row0, nrows, P.G, wave);
     };
-    if (nrows > 0) rq.load(qb, P.q_ls, P.q_hs, 0, nrows, P.G, P.D), rg.load(gb, P.g_ls, P.g_hs, 0, nrows, P.G, P.D), stats(0);
-    for (int row0 = 0; row0 < nrows; row0 += XA_TILE) {
-        __syncthreads();
-        rq.store(sq), rg.store(sg);
-        if (threadIdx.x < XA_TILE) sl[threadIdx.x] = rl, sd[threadIdx.x] = rd;
-        __syncthreads();
-        if (row0 + XA_TILE < nrows)
-            rq.load(qb, P.q_ls, P.q_hs, row0 + XA_TILE, nrows, P.G, P.D), rg.load(gb, P.g_ls, P.g_hs, row0 + XA_TILE, nrows, P.G, P.D), stats(row0 + XA_TILE);
+    const auto step = [&](int row0, int buf, const u16 *tq, const u16 *tg, u16 *nq, u16 *ng) {
+        if (threadIdx.x < XA_TILE) sl[buf][threadIdx.x] = rl == -INFINITY ? INFINITY : rl * XA_LOG2E, sd[buf][threadIdx.x] = rd;
+        xa_arrived();
+        if (row0 + XA_TILE < nrows) request(row0 + XA_TILE, nq, ng);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             f16v s = xa_zero16(), dp = xa_zero16();
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
-                s = PCM_MFMA16(lds_bf8(sq + (32 * j + col) * LD + 16 * t + 8 * h), kf[t], s);
-                dp = PCM_MFMA16(lds_bf8(sg + (32 * j + col) * LD + 16 * t + 8 * h), vf[t], dp);
+                s = PCM_MFMA16(xa_rows_operand<DP>(tq, 32 * j, t, lane), kf[t], s);
+                dp = PCM_MFMA16(xa_rows_operand<DP>(tg, 32 * j, t, lane), vf[t], dp);
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 l2 = *(const float4 *)(sl + 32 * j + 8 * g + 4 * h), de = *(const float4 *)(sd + 32 * j + 8 * g + 4 * h);
+                const float4 l2 = *(const float4 *)(sl[buf] + 32 * j + 8 * g + 4 * h), de = *(const float4 *)(sd[buf] + 32 * j + 8 * g + 4 * h);
                 const float a[4] = {l2.x, l2.y, l2.z, l2.w}, e[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -507,11 +645,20 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) pcm_xattn_dkv_kernel(XaP
                 const bf8 p = xa_pack(s, u), ds = xa_pack(dp, u);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) {
-                    dv[i] = PCM_MFMA16(xa_transposed<LD>(sg, 32 * j + 16 * u, i, lane), p, dv[i]);
-                    dk[i] = PCM_MFMA16(xa_transposed<LD>(sq, 32 * j + 16 * u, i, lane), ds, dk[i]);
+                    dv[i] = PCM_MFMA16(xa_transposed<DP>(tg, 32 * j + 16 * u, i, lane), p, dv[i]);
+                    dk[i] = PCM_MFMA16(xa_transposed<DP>(tq, 32 * j + 16 * u, i, lane), ds, dk[i]);
                 }
             }
         }
+    };
+    if (nrows > 0) {
+        request(0, sq0, sg0);
+        int row0 = 0;
+        for (; row0 + XA_TILE < nrows; row0 += 2 * XA_TILE) {
+            step(row0, 0, sq0, sg0, sq1, sg1);
+            step(row0 + XA_TILE, 1, sq1, sg1, sq0, sg0);
+        }
+        if (row0 < nrows) step(row0, 0, sq0, sg0, sq1, sg1);
     }
     if (!held) return;
     const long at = (key_row * P.Hkv + kvh) * P.D;
@@ -526,7 +673,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) pcm_xattn_dkv_kernel(XaP
     do {                                                                                                    \
         if ((P).D <= 32) hipLaunchKernelGGL((kernel<32>), dim3(grid), dim3(256), 0, s, P);                  \
         else if ((P).D <= 64) hipLaunchKernelGGL((kernel<64>), dim3(grid), dim3(256), 0, s, P);             \
-        else if ((P).D <= 96) hipLaunchKernelGGL((kernel<96>), dim3(grid), dim3(256), 0, s, P);             \
         else hipLaunchKernelGGL((kernel<128>), dim3(grid), dim3(256), 0, s, P);                             \
     } while (0)
 
@@ -538,18 +684,24 @@ long xa_tiles(int packed, int B, int len, long rows, int mult, int per)
     return packed ? (rows * mult + per - 1) / per + B + 1 : (long)B * (((long)len * mult + per - 1) / per);
 }
 
+// The forward pass of few rows (see pcm_xattn_few_kernel): every (sequence, key head) has 32 rows at most.  A packed side's longest
+// sequence is not known here: only its total counts.
+bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows : (long)L) * G <= 32; }
+
 // Splits of the keys.  A workgroup per (tile, key head) is too few for 256 compute units when the rows are few (one token of a rollout,
-// a decoder's 100 queries): the keys are then shared out until about 512 workgroups run, with at least 256 keys (4 tiles) each, since a
-// split writes and re-reads its row's fp32 sums.
-int xa_splits(int B, int H, int Hkv, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed)
+// a decoder's 100 queries): the keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and
+// re-reads its row's fp32 sums and costs a second launch (4 - 5 us), so it has 256 keys at least, in the few-row kernel, whose four waves share
+// a split's keys, 1024.
+int xa_splits(int B, int H, int Hkv, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, bool few)
 {
     const int G = H / Hkv;
     const long work = (q_packed ? (q_rows * G + XA_ROWS - 1) / XA_ROWS + B - 1 : xa_tiles(0, B, L, q_rows, G, XA_ROWS)) * Hkv;
-    const long keys = kv_packed ? (kv_rows + B - 1) / B : S;
-    long n = (512 + work - 1) / (work > 0 ? work : 1);
-    n = n < keys / 256 ? n : keys / 256;
+    const long keys = kv_packed ? (kv_rows + B - 1) / B : S, least = few ? 1024 : 256;
+    long n = 512 / (work > 0 ? work : 1);
+    n = n < keys / least ? n : keys / least;
     return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
+int xa_splits(const XaParams &P, bool few) { return xa_splits(P.B, P.H, P.Hkv, P.L, P.q_rows, P.q_off != nullptr, P.S, P.kv_rows, P.kv_off != nullptr, few); }
 
 bool xa_strides_ok(const void *p, long bs, long ls, long hs) { return (((uintptr_t)p) & 15) == 0 && ((bs | ls | hs) & 7) == 0; }
 
@@ -582,7 +734,7 @@ extern "C" long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, lon
 {
     if (B <= 0 || L < 0 || S < 0 || q_rows < 0 || kv_rows < 0 || !xa_shape_ok(H, Hkv, D)) return 0;
     if (!q_packed) q_rows = (long)B * L;
-    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed);
+    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed, false);  // the few-row kernel takes no more
     return n > 1 ? (long)n * q_rows * H * (D + 2) * 4 : 0;
 }
 
@@ -599,15 +751,22 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     if (bad) return bad;
     if (!out || (((uintptr_t)out | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
     P.out = (u16 *)out, P.lse = lse;
-    P.nsplit = xa_splits(B, H, Hkv, L, P.q_rows, q_offset != nullptr, S, P.kv_rows, kv_offset != nullptr);
+    const bool few = xa_few(L, P.q_rows, q_offset != nullptr, P.G);
+    P.nsplit = xa_splits(P, few);
     if (P.nsplit > 1) {
         if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * (D + 2) * 4) return PCM_ERR_BAD_ARG;
         P.part_o = (float *)ws, P.part_ml = (float *)ws + (long)P.nsplit * P.q_rows * H * D;
     }
     P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS);
     const hipStream_t s = (hipStream_t)stream;
-    XA_BY_DIM(pcm_xattn_fwd_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
-    if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_join_kernel, dim3((unsigned)((P.q_rows * H + 3) / 4)), dim3(256), 0, s, P);
+    if (few) XA_BY_DIM(pcm_xattn_few_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
+    else XA_BY_DIM(pcm_xattn_fwd_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
+    if (P.nsplit > 1) {
+        const long rows = P.q_rows * H;
+        if (D <= 32) hipLaunchKernelGGL((pcm_xattn_join_kernel<8>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, P);
+        else if (D <= 64) hipLaunchKernelGGL((pcm_xattn_join_kernel<16>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, P);
+        else hipLaunchKernelGGL((pcm_xattn_join_kernel<32>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, P);
+    }
     return PCM_LAUNCH_STATUS();
 }
 
@@ -631,15 +790,14 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
     P.delta = delta, P.dq = (u16 *)dq, P.dk = (u16 *)dk, P.dv = (u16 *)dv;
     const hipStream_t s = (hipStream_t)stream;
     if (P.q_rows > 0) {
-        P.nsplit = xa_splits(B, H, Hkv, L, P.q_rows, q_offset != nullptr, S, P.kv_rows, kv_offset != nullptr);
+        P.nsplit = xa_splits(P, false);
         if (P.nsplit > 1) {
             if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * D * 4) return PCM_ERR_BAD_ARG;
             P.part_o = (float *)ws;
         }
-        hipLaunchKernelGGL(pcm_xattn_delta_kernel, dim3((unsigned)((P.q_rows * H + 15) / 16)), dim3(256), 0, s, P);
         P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS);
         XA_BY_DIM(pcm_xattn_dq_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
-        if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_dq_join_kernel, dim3((unsigned)((P.q_rows * H * (D / 2) + 255) / 256)), dim3(256), 0, s, P);
+        if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_dq_join_kernel, dim3((unsigned)((P.q_rows * H * (D / 4) + 255) / 256)), dim3(256), 0, s, P);
     }
     if (P.kv_rows > 0) {
         P.tiles = (int)xa_tiles(kv_offset != nullptr, B, S, P.kv_rows, 1, XA_ROWS);
