@@ -114,17 +114,19 @@ __device__ __forceinline__ void xa_row_operand(const u16 *row, bool ok, int D, i
 
 // Tiles of 64 rows x DP channels in LDS, filled by global_load_lds: a wave's 64 16-byte pieces go to consecutive addresses, no registers
 // and no LDS write instructions.  That layout cannot be padded, so the piece a slot holds is permuted by its row (the lane picks its
-// source): the 8 lanes that read one piece of 8 neighbouring rows, and the 4 rows x 2 pieces of a 16-lane group of ds_read_b64_tr_b16, meet
-// different banks.  Pieces outside (absent or masked rows, channels from D on) are read from a block of zeros.
+// source), see xa_swz.  Pieces outside (absent or masked rows, channels from D on) are read from a block of zeros.
 __device__ uint4 xa_zeros;
 typedef __attribute__((address_space(3))) void *xa_lds_p;
 typedef const __attribute__((address_space(1))) void *xa_glb_p;
 
+// 64 banks of 4 bytes.  ds_read_b128 serves the lanes 0-3, 12-15, 20-23, 24-27 of 32 together, then the other 16: the rows of either set
+// that share a place modulo 256 bytes must hold a piece in different slots.  ds_read_b64_tr_b16 serves 32 lanes together, 64 bytes of
+// each of 4 neighbouring rows: those must lie in different 64-byte groups.  Both hold for these bit permutations of the row (counted:
+// SQ_LDS_BANK_CONFLICT was half of the LDS cycles with a permutation made for 8 neighbouring lanes).
 template <int DP>
-__device__ __forceinline__ int xa_swz(int r)
+__device__ __forceinline__ constexpr int xa_swz(int r)
 {
-    if constexpr (DP >= 64) return ((r & 3) << 1) | ((r >> 2) & 1);
-    else return (((r >> 1) & 1) << 1) | ((r >> 2) & 1);  // two rows in 128 bytes
+    return DP == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (DP == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : (r >> 2) & 3);
 }
 template <int DP>
 __device__ __forceinline__ int xa_at(int row, int piece)  // value offset of a piece inside a tile
@@ -138,12 +140,11 @@ struct XaStage {
     static constexpr int PIECES = DP / 8, NR = THREADS / PIECES, N = ROWS / NR;
     int r;        // tile row of the first piece
     int p;        // its channel
-    bool in;      // p < D
     int dim;
-    static_assert(NR % 8 == 0 || (NR == 4 && DP >= 64), "see load()");
+    static_assert((NR & (NR - 1)) == 0 && ROWS % NR == 0, "see load()");
     __device__ __forceinline__ void init(int t, int D)
     {
-        r = t / PIECES, p = 8 * ((t - r * PIECES) ^ xa_swz<DP>(r)), in = p < D, dim = D;
+        r = t / PIECES, p = 8 * ((t - r * PIECES) ^ xa_swz<DP>(r)), dim = D;
     }
     static __device__ __forceinline__ void put(const u16 *src, bool ok, u16 *tile, int n, int wave)
     {
@@ -156,9 +157,8 @@ struct XaStage {
         const unsigned long long mine = visible >> r;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            // the permutation repeats every 8 rows; 4 rows further it is its neighbour's
-            const int pn = NR % 8 != 0 && (n & 1) ? p ^ 8 : p;
-            put(src + n * (NR * ls) + pn, (NR % 8 != 0 ? pn < dim : in) && ((mine >> (n * NR)) & 1), tile, n, wave);
+            const int pn = p ^ (8 * xa_swz<DP>(n * NR));  // r < NR and NR is a power of two: the permutation's bits separate
+            put(src + n * (NR * ls) + pn, pn < dim && ((mine >> (n * NR)) & 1), tile, n, wave);
         }
     }
 };
@@ -171,9 +171,10 @@ struct XaRowStage : XaStage<DP, ROWS, 256> {
 #pragma unroll
         for (int i = 0; i < Base::N; ++i) {
             const int row = row0 + Base::r + i * Base::NR, tok = G == 1 ? row : row / G, g = row - tok * G;
-            const bool ok = Base::in && row < n;
-            Base::put(a + tok * a_ls + g * a_hs + Base::p, ok, ta, i, wave);
-            Base::put(b + tok * b_ls + g * b_hs + Base::p, ok, tb, i, wave);
+            const int pn = Base::p ^ (8 * xa_swz<DP>(i * Base::NR));
+            const bool ok = pn < Base::dim && row < n;
+            Base::put(a + tok * a_ls + g * a_hs + pn, ok, ta, i, wave);
+            Base::put(b + tok * b_ls + g * b_hs + pn, ok, tb, i, wave);
         }
     }
 };
@@ -690,18 +691,18 @@ bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows
 
 // Splits of the keys.  A workgroup per (tile, key head) is too few for 256 compute units when the rows are few (one token of a rollout,
 // a decoder's 100 queries): the keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and
-// re-reads its row's fp32 sums and costs a second launch (4 - 5 us), so it has 256 keys at least, in the few-row kernel, whose four waves share
-// a split's keys, 1024.
-int xa_splits(int B, int H, int Hkv, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, bool few)
+// re-reads its row's fp32 sums and costs a second launch (4 - 5 us), so it has 256 keys at least (for one row over 2051 keys, 8 heads: 10 us
+// with 8 splits, 20 with one).
+int xa_splits(int B, int H, int Hkv, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed)
 {
     const int G = H / Hkv;
     const long work = (q_packed ? (q_rows * G + XA_ROWS - 1) / XA_ROWS + B - 1 : xa_tiles(0, B, L, q_rows, G, XA_ROWS)) * Hkv;
-    const long keys = kv_packed ? (kv_rows + B - 1) / B : S, least = few ? 1024 : 256;
+    const long keys = kv_packed ? (kv_rows + B - 1) / B : S, least = 256;
     long n = 512 / (work > 0 ? work : 1);
     n = n < keys / least ? n : keys / least;
     return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
-int xa_splits(const XaParams &P, bool few) { return xa_splits(P.B, P.H, P.Hkv, P.L, P.q_rows, P.q_off != nullptr, P.S, P.kv_rows, P.kv_off != nullptr, few); }
+int xa_splits(const XaParams &P) { return xa_splits(P.B, P.H, P.Hkv, P.L, P.q_rows, P.q_off != nullptr, P.S, P.kv_rows, P.kv_off != nullptr); }
 
 bool xa_strides_ok(const void *p, long bs, long ls, long hs) { return (((uintptr_t)p) & 15) == 0 && ((bs | ls | hs) & 7) == 0; }
 
@@ -734,7 +735,7 @@ extern "C" long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, lon
 {
     if (B <= 0 || L < 0 || S < 0 || q_rows < 0 || kv_rows < 0 || !xa_shape_ok(H, Hkv, D)) return 0;
     if (!q_packed) q_rows = (long)B * L;
-    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed, false);  // the few-row kernel takes no more
+    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed);
     return n > 1 ? (long)n * q_rows * H * (D + 2) * 4 : 0;
 }
 
@@ -752,7 +753,7 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     if (!out || (((uintptr_t)out | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
     P.out = (u16 *)out, P.lse = lse;
     const bool few = xa_few(L, P.q_rows, q_offset != nullptr, P.G);
-    P.nsplit = xa_splits(P, few);
+    P.nsplit = xa_splits(P);
     if (P.nsplit > 1) {
         if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * (D + 2) * 4) return PCM_ERR_BAD_ARG;
         P.part_o = (float *)ws, P.part_ml = (float *)ws + (long)P.nsplit * P.q_rows * H * D;
@@ -790,7 +791,7 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
     P.delta = delta, P.dq = (u16 *)dq, P.dk = (u16 *)dk, P.dv = (u16 *)dv;
     const hipStream_t s = (hipStream_t)stream;
     if (P.q_rows > 0) {
-        P.nsplit = xa_splits(P, false);
+        P.nsplit = xa_splits(P);
         if (P.nsplit > 1) {
             if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * D * 4) return PCM_ERR_BAD_ARG;
             P.part_o = (float *)ws;

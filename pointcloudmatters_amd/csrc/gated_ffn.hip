@@ -89,14 +89,15 @@ __device__ uint4 gf_zeros;  // what pieces outside a matrix are read from
 // One operand's tile of GF_BK contracted values, ROWS values of the operand's own index.
 // COL false: [ROWS][32], contracted index contiguous, four 16-byte pieces a row.  COL true: [32][ROWS], ROWS / 8 pieces a row.
 // global_load_lds writes a wave's 64 pieces to consecutive addresses, so the layout cannot be padded; instead the piece a slot holds is
-// permuted (the lane picks its source): 8 lanes reading one piece of 8 neighbouring rows, and the 4 x 4 half pieces that a 16-lane group
-// of ds_read_b64_tr_b16 reads from 4 neighbouring contracted rows, then meet different banks.
+// permuted (the lane picks its source).  64 banks of 4 bytes: ds_read_b128 serves the lanes 0-3, 12-15, 20-23, 24-27 of 32 together, then the
+// other 16, and rows of 64 bytes share banks every 4, so the row's bits 2 and 3 pick the slot; ds_read_b64_tr_b16 serves 32 lanes together,
+// 64 bytes of each of 4 neighbouring contracted rows, which have to lie in different 64-byte groups.
 template <bool COL, int ROWS>
 struct GfTile {
     static constexpr int PIECES = COL ? ROWS / 8 : 4, SIZE = ROWS * GF_BK, LOADS = SIZE / 8 / 256;
     static __device__ __forceinline__ int swz(int r)
     {
-        if constexpr (!COL) return (r >> 1) & 3;
+        if constexpr (!COL) return (r >> 2) & 3;
         else if constexpr (ROWS >= 128) return (r & 3) << 2;
         else return ((r >> 1) & 1) << 2;
     }
