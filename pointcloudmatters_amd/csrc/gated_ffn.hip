@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int GF_BK = 32;
+constexpr int GF_BK = 64;  // contracted values of a step: 128 bytes of a row
 
 // A matrix of 2-byte values, rows at `ld`; rows from `split` on come from the second part (gate | up weights).
 struct GfMat {
@@ -86,23 +86,25 @@ typedef __attribute__((address_space(3))) void *gf_lds_p;
 typedef const __attribute__((address_space(1))) void *gf_glb_p;
 __device__ uint4 gf_zeros;  // what pieces outside a matrix are read from
 
-// One operand's tile of GF_BK contracted values, ROWS values of the operand's own index.
-// COL false: [ROWS][32], contracted index contiguous, four 16-byte pieces a row.  COL true: [32][ROWS], ROWS / 8 pieces a row.
+// One operand's tile of GF_BK contracted values, ROWS values of the operand's own index, requested by THREADS threads.
+// COL false: [ROWS][64], contracted index contiguous, eight 16-byte pieces a row.  COL true: [64][ROWS], ROWS / 8 pieces a row.
 // global_load_lds writes a wave's 64 pieces to consecutive addresses, so the layout cannot be padded; instead the piece a slot holds is
 // permuted (the lane picks its source).  64 banks of 4 bytes: ds_read_b128 serves the lanes 0-3, 12-15, 20-23, 24-27 of 32 together, then the
-// other 16, and rows of 64 bytes share banks every 4, so the row's bits 2 and 3 pick the slot; ds_read_b64_tr_b16 serves 32 lanes together,
-// 64 bytes of each of 4 neighbouring contracted rows, which have to lie in different 64-byte groups.
-template <bool COL, int ROWS>
+// other 16, and rows of 128 bytes share banks every other row, so three bits of the row pick the slot; ds_read_b64_tr_b16 serves 32 lanes
+// together, 64 bytes of each of 4 neighbouring contracted rows, which have to lie in different 64-byte groups.
+template <bool COL, int ROWS, int THREADS>
 struct GfTile {
-    static constexpr int PIECES = COL ? ROWS / 8 : 4, SIZE = ROWS * GF_BK, LOADS = SIZE / 8 / 256;
+    static constexpr int PIECES = COL ? ROWS / 8 : 8, SIZE = ROWS * GF_BK, LOADS = SIZE / 8 / THREADS;
     static __device__ __forceinline__ int swz(int r)
     {
-        if constexpr (!COL) return (r >> 2) & 3;
+        if constexpr (!COL) return (r >> 1) & 7;
         else if constexpr (ROWS >= 128) return (r & 3) << 2;
         else return ((r >> 1) & 1) << 2;
     }
-    // The thread's n-th piece stands n * NROWS tile rows below its first (the permutation is the same: NROWS is a multiple of 8).
-    static constexpr int NROWS = 256 / PIECES;
+    // The thread's n-th piece stands n * NROWS tile rows below its first (the permutation is the same: NROWS is a multiple of 16).
+    static constexpr int NROWS = THREADS / PIECES;
+    static_assert(COL || NROWS % 16 == 0, "the permutation repeats every 16 rows");
+    static_assert(!COL || NROWS % 4 == 0, "the permutation repeats every 4 rows");
     const u16 *base;  // the first piece at contracted index 0
     long step;        // values from one piece to the next
     int left, koff;   // COL false: matrix rows left from the first piece's on; true: 1 or 0, columns in or outside.  koff: contracted index inside the tile
@@ -117,14 +119,19 @@ struct GfTile {
             base = m.p0 + (left ? col : 0) + r * m.ld;
         } else {
             long row = i0 + r;
-            if (glu) row = (row >> 6) * 32 + (row & 31) + ((row & 32) ? m.split : 0);  // virtual row -> gate | up weight row
+            left = 0, each = NROWS;
+            if (glu) {  // virtual row -> gate | up weight row: 32 and 32 of every 64
+                row = (row >> 6) * 32 + (row & 31) + ((row & 32) ? m.split : 0);
+                if constexpr (NROWS % 64 == 0) each = NROWS / 2;
+            }
             const bool second = row >= m.split;
             const long rr = second ? row - m.split : row;
-            left = (int)((second ? m.rows1 : m.rows0) - rr), koff = 8 * c, each = glu ? NROWS / 2 : NROWS, step = each * m.ld;
+            left = (int)((second ? m.rows1 : m.rows0) - rr), koff = 8 * c, step = each * m.ld;
             base = (second ? m.p1 : m.p0) + rr * m.ld + 8 * c;
         }
     }
-    // the tile of contracted indices k .. k + 31 on its way into LDS
+    // the tile of contracted indices k .. k + 63 on its way into LDS
+    template <bool GLU>
     __device__ __forceinline__ void load(const GfMat &m, u16 *tile, long k, long kend) const
     {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -134,9 +141,16 @@ struct GfTile {
         const long at = COL ? k * m.ld + (second ? (long)(m.p1 - m.p0) - (long)m.split * m.ld : 0) : k;
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
-            const bool in = COL ? left && koff + n * NROWS < rest : n * each < left && koff < rest;
-            const u16 *src = in ? base + (at + n * step) : (const u16 *)&gf_zeros;
-            __builtin_amdgcn_global_load_lds((gf_glb_p)src, (gf_lds_p)(tile + (n * 256 + wave * 64) * 8), 16, 0, 0);
+            bool in = COL ? left && koff + n * NROWS < rest : n * each < left && koff < rest;
+            const u16 *src = base + (at + n * step);
+            if constexpr (GLU && !COL && NROWS % 64 != 0) {  // 32 rows a pass: gate and up rows alternate
+                static_assert(!(GLU && !COL) || NROWS % 64 == 0 || NROWS == 32, "a pass covers whole runs of 32");
+                const int f = (n >> 1) * 32;
+                in = f < left && koff < rest;
+                src = base + (at + f * m.ld + ((n & 1) ? (long)(m.p1 - m.p0) : 0));
+            }
+            __builtin_amdgcn_global_load_lds((gf_glb_p)(in ? (const void *)src : (const void *)&gf_zeros),
+                                             (gf_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, 0, 0);
         }
     }
     // operand of rows i .. i + 31, contracted values 16 kk .. + 15
@@ -155,35 +169,29 @@ struct GfTile {
     }
 };
 
-// vmcnt(N) lgkmcnt(0): all but the wave's last N requests have arrived, its LDS reads are done
-template <int N>
-__device__ __forceinline__ void gf_wait()
+// The tile engine.  2 x WN waves; a wave owns MI x NI tiles of 32 x 32.  Two LDS buffers of 64 contracted values each: once tile t has arrived,
+// tile t + 1 is requested into the other buffer (global_load_lds: no registers, no LDS write instructions) and the step's matrix
+// instructions run meanwhile; one barrier a step.  A step takes 128 bytes of a row because that is a cache line: with steps of 64 bytes
+// the other half of every line had left the 32 KB cache before its turn, the lines went through it twice, and 256 x 128 tiles kept the
+// matrix cores at half of what they do here.  The buffers are two variables, so that the compiler can tell the reads of one from the requests into
+// the other and inserts no wait of its own between them.
+template <int EP, bool ACOL, bool BCOL, int MI, int NI, int WN>
+__global__ void __launch_bounds__(128 * WN, 2) pcm_gated_gemm_kernel(GfParams P)
 {
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
-}
-
-// The tile engine.  4 waves, 2 x 2; a wave owns MI x NI tiles of 32 x 32.  Three LDS buffers of 32 contracted values each: in step t all
-// operands of tile t come out of LDS, tile t + 2's pieces are requested straight into the buffer that step t - 1 read
-// (global_load_lds: no registers, no LDS write instructions), then the step's matrix instructions run.  One barrier a step, which waits
-// for tile t alone: tile t + 1 stays in flight.  (With one tile in flight a step took 2800 clocks for two workgroups on a compute unit, 1024 of
-// matrix work: every tile row's first reader waits for memory, and the others with it.)  The buffers are three variables, so that the
-// compiler can tell the reads of one from the requests into another and inserts no wait of its own between them.
-template <int EP, bool ACOL, bool BCOL, int MI, int NI>
-__global__ void __launch_bounds__(256, 2) pcm_gated_gemm_kernel(GfParams P)
-{
-    constexpr int BM = 64 * MI, BN = 64 * NI, COLS = 32 * NI, SLAB = COLS + 4;
-    typedef GfTile<ACOL, BM> TA;
-    typedef GfTile<BCOL, BN> TB;
-    constexpr int STAGE = (TA::SIZE + TB::SIZE) * 2, BYTES = STAGE > 2 * 32 * SLAB * 4 ? STAGE : 2 * 32 * SLAB * 4, LOADS = TA::LOADS + TB::LOADS;
-    __shared__ __attribute__((aligned(1024))) unsigned char sm0[BYTES], sm1[BYTES], sm2[BYTES];
+    constexpr int THREADS = 128 * WN, BM = 64 * MI, BN = 32 * NI * WN, COLS = 32 * NI, SLAB = COLS + 4;
+    typedef GfTile<ACOL, BM, THREADS> TA;
+    typedef GfTile<BCOL, BN, THREADS> TB;
+    constexpr int STAGE = (TA::SIZE + TB::SIZE) * 2, BYTES = STAGE > WN * 32 * SLAB * 4 ? STAGE : WN * 32 * SLAB * 4;
+    __shared__ __attribute__((aligned(1024))) unsigned char sm0[BYTES], sm1[BYTES];
     const int M = (int)P.M, N = (int)P.N;
     const long mt = (P.M + BM - 1) / BM, nt = (P.N + BN - 1) / BN, items = mt * nt * P.nsplit, per = (items + 7) / 8;
     const long item = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);  // one XCD's L2 sees consecutive tiles
-    if (item >= items) return;
+    if ((long)(blockIdx.x >> 3) >= per || item >= items) return;
     const long m0 = item / nt % mt * BM, n0 = item % nt * BN, split = item / (nt * mt);
     const long kt = (P.K + GF_BK - 1) / GF_BK, kper = (kt + P.nsplit - 1) / P.nsplit * GF_BK;
     const long k0 = split * kper, kend = k0 + kper < P.K ? k0 + kper : P.K;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = (wave >> 1) * 32 * MI, wn = (wave & 1) * COLS;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wm = (wave / WN) * 32 * MI, wn = (wave % WN) * COLS;
     f16v acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -192,49 +200,41 @@ __global__ void __launch_bounds__(256, 2) pcm_gated_gemm_kernel(GfParams P)
     TA ga;
     TB gb;
     ga.init(P.a, m0, false), gb.init(P.b, n0, EP == EP_GLU);
-    // every step requests a tile, behind the end one of zeros: the count of requests in flight stays the same
     const auto request = [&](unsigned char *sm, long k) {
-        ga.load(P.a, (u16 *)sm, k, kend), gb.load(P.b, (u16 *)sm + TA::SIZE, k, kend);
+        ga.template load<false>(P.a, (u16 *)sm, k, kend), gb.template load<EP == EP_GLU>(P.b, (u16 *)sm + TA::SIZE, k, kend);
     };
-    const auto step = [&](const unsigned char *cur, unsigned char *free, long k) {
-        gf_wait<LOADS>();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+    const auto step = [&](const unsigned char *cur, unsigned char *other, long k) {
+        __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0): this wave's pieces have arrived, its reads of the other buffer are done
+        __syncthreads();                   // ... and everybody's
+        if (k + GF_BK < kend) request(other, k + GF_BK);
+        __builtin_amdgcn_sched_barrier(0);  // the requests stay in front of the step's products, which they are to hide behind
         const u16 *ta = (const u16 *)cur, *tb = ta + TA::SIZE;
-        bf8 a[2][MI], b[2][NI];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
+        for (int kk = 0; kk < GF_BK / 16; ++kk) {
+            bf8 a[MI], b[NI];
 #pragma unroll
-            for (int i = 0; i < MI; ++i) a[kk][i] = TA::operand(ta, wm + 32 * i, kk, lane);
+            for (int i = 0; i < MI; ++i) a[i] = TA::operand(ta, wm + 32 * i, kk, lane);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) b[kk][j] = TB::operand(tb, wn + 32 * j, kk, lane);
-        }
-        request(free, k + 2 * GF_BK);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+            for (int j = 0; j < NI; ++j) b[j] = TB::operand(tb, wn + 32 * j, kk, lane);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = PCM_MFMA16(a[kk][i], b[kk][j], acc[i][j]);
+                for (int j = 0; j < NI; ++j) acc[i][j] = PCM_MFMA16(a[i], b[j], acc[i][j]);
+        }
     };
     if (k0 < kend) {
         request(sm0, k0);
-        request(sm1, k0 + GF_BK);
         long k = k0;
-        for (; k + 2 * GF_BK < kend; k += 3 * GF_BK) {
-            step(sm0, sm2, k);
+        for (; k + GF_BK < kend; k += 2 * GF_BK) {
+            step(sm0, sm1, k);
             step(sm1, sm0, k + GF_BK);
-            step(sm2, sm1, k + 2 * GF_BK);
         }
-        if (k < kend) step(sm0, sm2, k);
-        if (k + GF_BK < kend) step(sm1, sm0, k + GF_BK);
+        if (k < kend) step(sm0, sm1, k);
     }
-    gf_wait<0>();  // the last requests (of zeros) must not land in the slabs
     __syncthreads();
     // Epilogue: 32 rows at a time through a slab of the wave's own (an accumulator holds a column a lane), out of it 8 neighbouring
     // columns a lane, the same ones in every pass: 16-byte accesses to everything that is read and written beside the products.
-    float *const slab = (float *)(wave < 2 ? sm0 : sm1) + (wave & 1) * 32 * SLAB;
+    float *const slab = (float *)(wave < WN ? sm0 : sm1) + (wave % WN) * 32 * SLAB;
     constexpr int GROUPS = EP == EP_GLU ? 4 : COLS / 8;  // groups of 8 columns a row
     static_assert(64 % GROUPS == 0, "a lane's columns are the same in every pass");
     const int c = 8 * (lane % GROUPS), r0 = lane / GROUPS, col = (int)(EP == EP_GLU ? (n0 + wn) / 2 : n0 + wn) + c;
@@ -246,15 +246,29 @@ __global__ void __launch_bounds__(256, 2) pcm_gated_gemm_kernel(GfParams P)
         bias0[e] = (EP == EP_GLU || EP == EP_OUT) && P.bias0 && P.nsplit == 1 && col + e < width ? bf2f(P.bias0[col + e]) : 0.f;
         bias1[e] = EP == EP_GLU && P.bias1 && col + e < width ? bf2f(P.bias1[col + e]) : 0.f;
     }
+    constexpr int PASSES = 32 * GROUPS / 64;
+    uint4 ea[2][EP == EP_DGLU ? PASSES : 1], eu[2][EP == EP_DGLU ? PASSES : 1];
+    const auto fetch = [&](int i) {  // a and u of slab i, requested one slab ahead
+#pragma unroll
+        for (int g = 0; g < PASSES; ++g) {
+            // rows and columns outside are read from the last ones inside: no branch that the loads could sink into
+            const long row = min(m0 + wm + 32 * i + r0 + g * (64 / GROUPS), P.M - 1), at = row * P.Fp + min((long)col, P.Fp - 8);
+            ea[i & 1][g] = *(const uint4 *)(P.ea + at), eu[i & 1][g] = *(const uint4 *)(P.eu + at);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (EP == EP_DGLU) fetch(0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
+        if constexpr (EP == EP_DGLU)
+            if (i + 1 < MI) fetch(i + 1);
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) slab[crow(r, lane) * SLAB + 32 * j + (lane & 31)] = acc[i][j][r];
         __builtin_amdgcn_wave_barrier();  // the wave's LDS operations complete in order
 #pragma unroll
-        for (int g = 0; g < 32 * GROUPS / 64; ++g) {
+        for (int g = 0; g < PASSES; ++g) {
             const int r = r0 + g * (64 / GROUPS);
             const long row = m0 + wm + 32 * i + r;
             if ((int)row >= M) continue;
@@ -276,7 +290,7 @@ __global__ void __launch_bounds__(256, 2) pcm_gated_gemm_kernel(GfParams P)
             } else if constexpr (EP == EP_DGLU) {
                 if (col >= P.Fp) continue;
                 float a[8], u[8];
-                gf_f8(*(const uint4 *)(P.ea + row * P.Fp + col), a), gf_f8(*(const uint4 *)(P.eu + row * P.Fp + col), u);
+                gf_f8(ea[i & 1][g], a), gf_f8(eu[i & 1][g], u);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float2 g2 = gf_act_grad(a[e], P.act);
@@ -320,29 +334,15 @@ __global__ void __launch_bounds__(256, 2) pcm_gated_gemm_kernel(GfParams P)
         for (int e = 0; e < 8; ++e)
             for (int d = GROUPS; d < 64; d <<= 1) bias0[e] += __shfl_xor(bias0[e], d), bias1[e] += __shfl_xor(bias1[e], d);
         if (lane >= GROUPS || col >= P.Fp) return;
-        float *o = P.part + (m0 / (32 * MI) + (wave >> 1)) * 2 * P.Fp + col;
+        float *o = P.part + (m0 / (32 * MI) + wave / WN) * 2 * P.Fp + col;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = bias0[e], o[P.Fp + e] = bias1[e];
     }
 }
 
-// out = sum of the splits in split order (+ bias)
-__global__ void __launch_bounds__(256) pcm_gated_join_kernel(GfParams P)
-{
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= P.M * P.N) return;
-    const long row = i / P.N, n = i - row * P.N;
-    const bool second = row >= P.osplit;
-    const long rr = second ? row - P.osplit : row;
-    if (rr >= P.F) return;
-    float s = P.bias0 ? bf2f(P.bias0[n]) : 0.f;
-    for (int k = 0; k < P.nsplit; ++k) s += P.part[(long)k * P.M * P.N + i];
-    (second ? P.out1 : P.out)[rr * P.ldo + n] = gf_bf(s);
-}
-
 // Bias gradients.  The sums of da | du over a wave's rows leave the epilogue that forms them (one partial row per wave row: reading
-// da | du again would cost as much as writing it); dy is summed here, `slots` partial rows of fixed row ranges.  Then one wave per 16
-// columns, 4 lanes per column over interleaved partial rows, joined by two exchanges: the order never changes.
+// da | du again would cost as much as writing it); dy is summed here, `slots` partial rows of fixed row ranges.  pcm_gated_close_kernel
+// sums the partial rows; the order never changes.
 struct GfSums {
     const u16 *g;
     long ld, rows;
@@ -365,23 +365,80 @@ __global__ void __launch_bounds__(256) pcm_gated_colsum_kernel(GfSums P)
     }
     *(float2 *)(P.part1 + (long)blockIdx.y * P.C[1] + c) = make_float2(a, b);
 }
-__global__ void __launch_bounds__(256) pcm_gated_colsum_join_kernel(GfSums P)
+// What closes a pass, in one launch: split contractions summed in split order (+ bias), four values a thread, and the bias gradients'
+// partial rows, 16 columns and 16 interleaved row lanes a workgroup.
+struct GfJoin {
+    const float *part;
+    u16 *out, *out1;
+    const u16 *bias;
+    long M, N, osplit, F, ldo, end;  // end: running count of workgroups
+    int nsplit;
+};
+struct GfClose {
+    GfJoin j[3];
+    int n;
+    GfSums s;
+    int sums;  // workgroups of the first part's columns (da | du), then of the second's (dy)
+};
+__global__ void __launch_bounds__(256) pcm_gated_close_kernel(GfClose P)
 {
-    const int j = blockIdx.y, lane = threadIdx.x & 63, c = ((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6)) * 16 + (lane & 15);
+    __shared__ float lds[4][16];
+    long blk = blockIdx.x;
+    int j = 0;
+    while (j < P.n && blk >= P.j[j].end) ++j;
+    if (j < P.n) {
+        const GfJoin &J = P.j[j];
+        const long i = ((blk - (j ? P.j[j - 1].end : 0)) * 256 + threadIdx.x) * 4, size = J.M * J.N;
+        if (i >= size) return;
+        if (J.N % 4 == 0) {
+            const long row = i / J.N, n = i - row * J.N;
+            const bool second = row >= J.osplit;
+            const long rr = second ? row - J.osplit : row;
+            if (rr >= J.F) return;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int k = 0; k < J.nsplit; ++k) {
+                const float4 v = *(const float4 *)(J.part + k * size + i);
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            if (J.bias) s.x += bf2f(J.bias[n]), s.y += bf2f(J.bias[n + 1]), s.z += bf2f(J.bias[n + 2]), s.w += bf2f(J.bias[n + 3]);
+            u16 *o = (second ? J.out1 : J.out) + rr * J.ldo + n;
+            if (((uintptr_t)o & 7) == 0) *(uint2 *)o = make_uint2(cvt_pk_bf16(s.x, s.y), cvt_pk_bf16(s.z, s.w));
+            else o[0] = gf_bf(s.x), o[1] = gf_bf(s.y), o[2] = gf_bf(s.z), o[3] = gf_bf(s.w);
+            return;
+        }
+        for (long e = i; e < i + 4 && e < size; ++e) {
+            const long row = e / J.N, n = e - row * J.N;
+            const bool second = row >= J.osplit;
+            const long rr = second ? row - J.osplit : row;
+            if (rr >= J.F) continue;
+            float s = 0.f;
+#pragma unroll 4
+            for (int k = 0; k < J.nsplit; ++k) s += J.part[k * size + e];
+            (second ? J.out1 : J.out)[rr * J.ldo + n] = gf_bf(s + (J.bias ? bf2f(J.bias[n]) : 0.f));
+        }
+        return;
+    }
+    blk -= P.n ? P.j[P.n - 1].end : 0;
+    const int part = blk >= P.sums, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)(blk - (part ? P.sums : 0)) * 16 + (lane & 15);
+    const GfSums &S = P.s;
     float s = 0.f;
-    if (c < P.C[j]) {
+    if (c < S.C[part]) {
 #pragma unroll 8
-        for (int k = lane >> 4; k < P.slots[j]; k += 4) s += P.part[j][(long)k * P.C[j] + c];
+        for (int k = wave * 4 + (lane >> 4); k < S.slots[part]; k += 16) s += S.part[part][(long)k * S.C[part] + c];
     }
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
-    if (lane >= 16 || c >= P.C[j]) return;
-    if (j == 1) {
-        if (c < P.E) P.out[2][c] = gf_bf(s);
-    } else if (c < P.F) {
-        P.out[0][c] = gf_bf(s);
-    } else if (c >= P.Fp && c - P.Fp < P.F) {
-        P.out[1][c - P.Fp] = gf_bf(s);
+    if (lane < 16) lds[wave][lane] = s;
+    __syncthreads();
+    if (threadIdx.x >= 16 || c >= S.C[part]) return;
+    s = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
+    if (part) {
+        if (c < S.E) S.out[2][c] = gf_bf(s);
+    } else if (c < S.F) {
+        S.out[0][c] = gf_bf(s);
+    } else if (c >= S.Fp && c - S.Fp < S.F) {
+        S.out[1][c - S.Fp] = gf_bf(s);
     }
 }
 
@@ -544,27 +601,46 @@ struct GfPacker {
 GfMat gf_mat(const u16 *p, long ld, long rows, long cols) { return GfMat{p, p, ld, 0x7FFFFFFF, (int)rows, 0, (int)cols}; }
 GfMat gf_mat2(const u16 *p0, const u16 *p1, long ld, long split, long rows, long cols) { return GfMat{p0, p1, ld, (int)split, (int)rows, (int)rows, (int)cols}; }
 
-long gf_tiles(long M, long N, int mi, int ni) { return (M + 64 * mi - 1) / (64 * mi) * ((N + 64 * ni - 1) / (64 * ni)); }
+// Tiles: 256 x 256 (8 waves of 128 x 64, one workgroup a compute unit), 128 x 128 and 64 x 128 (4 waves, two or three a compute unit).
+struct GfShape {
+    int bm, bn;
+};
+constexpr GfShape GF_LARGE{256, 256}, GF_MIDDLE{128, 128}, GF_SMALL{64, 128};
+long gf_tiles(long M, long N, GfShape s) { return (M + s.bm - 1) / s.bm * ((N + s.bn - 1) / s.bn); }
 
-template <int EP, bool ACOL, bool BCOL, int MI, int NI>
-void gf_launch_tile(const GfParams &P, hipStream_t s)
+// The shape of a product's tiles: large ones pass the least data per product through LDS and cache, but a launch of 257 of them takes as long as one
+// of 512.  Taken: the largest shape whose last round of workgroups is not mostly empty (256 compute units, 1 / 2 / 3 workgroups each); over a short
+// contraction the smaller ones, of which one multiplies while its neighbour is in the epilogue.
+GfShape gf_shape(long M, long N, long K, int nsplit)
 {
-    hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, MI, NI>), dim3((unsigned)gf_up(gf_tiles(P.M, P.N, MI, NI) * P.nsplit, 8)), dim3(256), 0, s, P);
+    const long large = gf_tiles(M, N, GF_LARGE) * nsplit, middle = gf_tiles(M, N, GF_MIDDLE) * nsplit;
+    if (K / nsplit >= 1024 && large >= 200 && large * 10 >= (large + 255) / 256 * 256 * 7) return GF_LARGE;
+    return middle >= 256 ? GF_MIDDLE : GF_SMALL;
 }
-
-// Tile of a product: the largest that gives every compute unit a workgroup or two.  A wave of 128 x 64 reads 12 operand pieces for 16
-// matrix instructions, one of 32 x 64 six for four: large tiles are bound by the matrix cores, small ones by LDS, but 52 workgroups of
-// the large kind leave four fifths of the chip idle.
-int gf_tile_mi(long M, long N, int nsplit) { return gf_tiles(M, N, 4, 2) * nsplit >= 400 ? 4 : (gf_tiles(M, N, 2, 2) * nsplit >= 256 ? 2 : 1); }
 
 template <int EP, bool ACOL, bool BCOL>
 void gf_launch(const GfParams &P, hipStream_t s)
 {
-    const int mi = gf_tile_mi(P.M, P.N, P.nsplit);
-    if (mi == 4) gf_launch_tile<EP, ACOL, BCOL, 4, 2>(P, s);
-    else if (mi == 2) gf_launch_tile<EP, ACOL, BCOL, 2, 2>(P, s);
-    else gf_launch_tile<EP, ACOL, BCOL, 1, 2>(P, s);
-    if (P.nsplit > 1) hipLaunchKernelGGL(pcm_gated_join_kernel, dim3((unsigned)((P.M * P.N + 255) / 256)), dim3(256), 0, s, P);
+    const GfShape t = gf_shape(P.M, P.N, P.K, P.nsplit);
+    const dim3 grid((unsigned)((gf_tiles(P.M, P.N, t) * P.nsplit + 7) / 8 * 8));
+    if (t.bm == 256) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 4, 2, 4>), grid, dim3(512), 0, s, P);
+    else if (t.bm == 128) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 2, 2, 2>), grid, dim3(256), 0, s, P);
+    else hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 1, 2, 2>), grid, dim3(256), 0, s, P);
+}
+
+// adds a product's joining to what closes the pass
+void gf_join(GfClose &c, const GfParams &P)
+{
+    if (P.nsplit <= 1) return;
+    GfJoin &j = c.j[c.n++];
+    j = GfJoin{P.part, P.out, P.out1, P.bias0, P.M, P.N, P.osplit, P.F, P.ldo, 0, P.nsplit};
+    j.end = (c.n > 1 ? c.j[c.n - 2].end : 0) + (P.M * P.N + 1023) / 1024;
+}
+void gf_close(GfClose &c, hipStream_t s)
+{
+    c.sums = (c.s.C[0] + 15) / 16;
+    const long blocks = (c.n ? c.j[c.n - 1].end : 0) + c.sums + (c.s.C[1] + 15) / 16;
+    if (blocks) hipLaunchKernelGGL(pcm_gated_close_kernel, dim3((unsigned)blocks), dim3(256), 0, s, c);
 }
 
 // Splits of a product's contraction where its output has too few tiles: weight gradients contract over all rows, the outer products of
@@ -572,24 +648,24 @@ void gf_launch(const GfParams &P, hipStream_t s)
 // re-reads the fp32 output).
 int gf_splits(long M, long N, long K)
 {
-    const long tiles = gf_tiles(M, N, 4, 2) >= 64 ? gf_tiles(M, N, 4, 2) : (gf_tiles(M, N, 2, 2) >= 64 ? gf_tiles(M, N, 2, 2) : gf_tiles(M, N, 1, 2));
+    const long middle = gf_tiles(M, N, GF_MIDDLE), tiles = middle >= 64 ? middle : gf_tiles(M, N, GF_SMALL);
     if (tiles >= 256) return 1;
-    long n = (512 + tiles - 1) / tiles;
+    long n = 512 / tiles;
     n = n < K / 256 ? n : K / 256;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
 long gf_part_bytes(long M, long N, long K) { const int n = gf_splits(M, N, K); return n > 1 ? gf_up(n * M * N * 4, 256) : 0; }
 
-// the backward products run one after another and share one buffer of partial sums
+// partial sums of the three backward products, joined together at the end
 long gf_back_part_bytes(long R, int E, int F)
 {
-    const long Fp = gf_up(F, 64), a = gf_part_bytes(2 * Fp, E, R), b = gf_part_bytes(E, F, R), c = gf_part_bytes(R, E, 2 * Fp);
-    return a > b ? (a > c ? a : c) : (b > c ? b : c);
+    const long Fp = gf_up(F, 64);
+    return gf_part_bytes(R, E, 2 * Fp) + gf_part_bytes(2 * Fp, E, R) + gf_part_bytes(E, F, R);
 }
-int gf_slots(long R) { return (int)(R < 64 ? 1 : (R / 32 > 128 ? 128 : R / 32)); }
+int gf_slots(long R) { return (int)(R < 64 ? 1 : (R / 32 > 512 ? 512 : R / 32)); }
 // partial rows of da | du: two wave rows per tile row
-long gf_wave_rows(long R, long Fp) { const int mi = gf_tile_mi(R, Fp, 1); return (R + 64 * mi - 1) / (64 * mi) * 2; }
-long gf_sum_bytes(long R, int E, long Fp) { return gf_up((gf_wave_rows(R, Fp) * 2 * Fp + gf_slots(R) * gf_up(E, 8)) * 4, 256); }
+long gf_wave_rows(long R, int E, long Fp) { const int bm = gf_shape(R, Fp, gf_up(E, 8), 1).bm; return (R + bm - 1) / bm * 2; }
+long gf_sum_bytes(long R, int E, long Fp) { return gf_up((gf_wave_rows(R, E, Fp) * 2 * Fp + gf_slots(R) * gf_up(E, 8)) * 4, 256); }
 bool gf_sizes_ok(long R, int E, int F) { return R <= 0x3FFFFFFFL && E <= (1 << 20) && F <= (1 << 20); }
 long gf_pack_bytes(long rows, int cols) { return gf_up(rows * gf_up(cols, 8) * 2, 256); }
 
@@ -656,6 +732,9 @@ extern "C" int pcm_gated_ffn_forward_hip(long R, int E, int F, int act, const vo
     Q.a = gf_mat((const u16 *)h, Fp, R, Fp), Q.b = gf_mat(pd, ldd, E, gf_up(F, 8));
     Q.M = R, Q.N = E, Q.K = gf_up(F, 8), Q.nsplit = gf_splits(R, E, Q.K), Q.part = part, Q.bias0 = (const u16 *)bd, Q.F = Q.osplit = R, Q.out = (u16 *)y, Q.ldo = E;
     gf_launch<EP_OUT, false, false>(Q, s);
+    GfClose c{};
+    gf_join(c, Q);
+    gf_close(c, s);
     return PCM_LAUNCH_STATUS();
 }
 
@@ -675,8 +754,9 @@ extern "C" int pcm_gated_ffn_backward_hip(long R, int E, int F, int act, const v
     char *at = (char *)ws + gf_up(R * 2 * Fp * 2, 256);
     float *sums = (float *)at;
     at += gf_sum_bytes(R, E, Fp);
-    float *part = (float *)at;
+    float *const part_dx = (float *)at, *const part_w1 = part_dx + gf_part_bytes(R, E, 2 * Fp) / 4, *const part_w2 = part_w1 + gf_part_bytes(2 * Fp, E, R) / 4;
     at += gf_back_part_bytes(R, E, F);
+    GfClose c{};
     GfPacker pk(at, (char *)ws + ws_bytes - at);
     long ldx = x_ls, ldy = dy_ls, ldg = E, ldu = E, ldd = F;
     const u16 *py = pk.get(dy, R, E, ldy), *px = dwg ? pk.get(x, R, E, ldx) : nullptr;
@@ -694,31 +774,33 @@ extern "C" int pcm_gated_ffn_backward_hip(long R, int E, int F, int act, const v
     if (dx) {
         GfParams P{};
         P.a = gf_mat(dau, 2 * Fp, R, 2 * Fp), P.b = gf_mat2(pg, pu, ldg, Fp, F, Ep);
-        P.M = R, P.N = E, P.K = 2 * Fp, P.nsplit = gf_splits(P.M, P.N, P.K), P.part = part, P.F = P.osplit = R, P.out = (u16 *)dx, P.ldo = E;
+        P.M = R, P.N = E, P.K = 2 * Fp, P.nsplit = gf_splits(P.M, P.N, P.K), P.part = part_dx, P.F = P.osplit = R, P.out = (u16 *)dx, P.ldo = E;
         gf_launch<EP_OUT, false, true>(P, s);
+        gf_join(c, P);
     }
     if (dwg) {
         GfParams P{};
         P.a = gf_mat(dau, 2 * Fp, R, 2 * Fp), P.b = gf_mat(px, ldx, R, Ep);
-        P.M = 2 * Fp, P.N = E, P.K = R, P.nsplit = gf_splits(P.M, P.N, P.K), P.F = F, P.out = (u16 *)dwg, P.out1 = (u16 *)dwu, P.ldo = E, P.part = part;
+        P.M = 2 * Fp, P.N = E, P.K = R, P.nsplit = gf_splits(P.M, P.N, P.K), P.F = F, P.out = (u16 *)dwg, P.out1 = (u16 *)dwu, P.ldo = E, P.part = part_w1;
         P.osplit = Fp;
         gf_launch<EP_WGRAD, true, true>(P, s);
+        gf_join(c, P);
     }
     if (dwd) {
         GfParams P{};
         P.a = gf_mat(py, ldy, R, Ep), P.b = gf_mat((const u16 *)h, Fp, R, Fp);
-        P.M = E, P.N = F, P.K = R, P.nsplit = gf_splits(P.M, P.N, P.K), P.F = E, P.osplit = E, P.out = (u16 *)dwd, P.ldo = F, P.part = part;
+        P.M = E, P.N = F, P.K = R, P.nsplit = gf_splits(P.M, P.N, P.K), P.F = E, P.osplit = E, P.out = (u16 *)dwd, P.ldo = F, P.part = part_w2;
         gf_launch<EP_WGRAD, true, true>(P, s);
+        gf_join(c, P);
     }
     if (dbg || dbd) {
-        GfSums P{};
+        GfSums &P = c.s;
         P.rows = R, P.E = E, P.F = F, P.Fp = (int)Fp, P.g = py, P.ld = ldy;
-        P.slots[0] = (int)gf_wave_rows(R, Fp), P.C[0] = dbg ? (int)(2 * Fp) : 0, P.part[0] = sums;
+        P.slots[0] = (int)gf_wave_rows(R, E, Fp), P.C[0] = dbg ? (int)(2 * Fp) : 0, P.part[0] = sums;
         P.slots[1] = gf_slots(R), P.C[1] = dbd ? (int)Ep : 0, P.part1 = sums + P.slots[0] * 2 * Fp, P.part[1] = P.part1;
         P.out[0] = (u16 *)dbg, P.out[1] = (u16 *)dbu, P.out[2] = (u16 *)dbd;
         if (dbd) hipLaunchKernelGGL(pcm_gated_colsum_kernel, dim3((unsigned)((Ep + 511) / 512), P.slots[1]), dim3(256), 0, s, P);
-        const long widest = P.C[0] > P.C[1] ? P.C[0] : P.C[1];
-        hipLaunchKernelGGL(pcm_gated_colsum_join_kernel, dim3((unsigned)((widest + 63) / 64), 2), dim3(256), 0, s, P);
     }
+    gf_close(c, s);
     return PCM_LAUNCH_STATUS();
 }
