@@ -131,8 +131,9 @@ struct GfTile {
         }
     }
     // the tile of contracted indices k .. k + 63 on its way into LDS
+    // (its pieces n0 .. n1 - 1)
     template <bool GLU>
-    __device__ __forceinline__ void load(const GfMat &m, u16 *tile, long k, long kend) const
+    __device__ __forceinline__ void load(const GfMat &m, u16 *tile, long k, long kend, int n0 = 0, int n1 = LOADS) const
     {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
         // a tile never straddles the parts: `split` is a multiple of 64
@@ -140,7 +141,7 @@ struct GfTile {
         const int rest = (int)((COL ? min(kend, second ? m.split + (long)m.rows1 : (long)m.rows0) : kend) - k);
         const long at = COL ? k * m.ld + (second ? (long)(m.p1 - m.p0) - (long)m.split * m.ld : 0) : k;
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) {
+        for (int n = n0; n < n1; ++n) {
             bool in = COL ? left && koff + n * NROWS < rest : n * each < left && koff < rest;
             const u16 *src = base + (at + n * step);
             if constexpr (GLU && !COL && NROWS % 64 != 0) {  // 32 rows a pass: gate and up rows alternate
@@ -206,20 +207,40 @@ __global__ void __launch_bounds__(128 * WN, 2) pcm_gated_gemm_kernel(GfParams P)
     const auto step = [&](const unsigned char *cur, unsigned char *other, long k) {
         __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0): this wave's pieces have arrived, its reads of the other buffer are done
         __syncthreads();                   // ... and everybody's
-        if (k + GF_BK < kend) request(other, k + GF_BK);
-        __builtin_amdgcn_sched_barrier(0);  // the requests stay in front of the step's products, which they are to hide behind
         const u16 *ta = (const u16 *)cur, *tb = ta + TA::SIZE;
+        // One workgroup a compute unit (8 waves): all requests at once would hold up every wave's first products until the last is
+        // accepted (0.6 us for 64 KB), so they are spread over the step's first half.  With two or three workgroups the others multiply
+        // meanwhile, and the earliest request is best: 128 x 128 tiles took 8 % longer with spread requests, 256 x 256 ones 12 % less.
+        constexpr bool SPREAD = WN == 4;
+        constexpr int KK = GF_BK / 16, ALL = TA::LOADS + TB::LOADS, SLOTS = 2 * MI;
+        if (!SPREAD) {
+            if (k + GF_BK < kend) request(other, k + GF_BK);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        bf8 a[2][MI], b[2][NI];
+        const auto read = [&](int kk) {
 #pragma unroll
-        for (int kk = 0; kk < GF_BK / 16; ++kk) {
-            bf8 a[MI], b[NI];
+            for (int i = 0; i < MI; ++i) a[kk & 1][i] = TA::operand(ta, wm + 32 * i, kk, lane);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) a[i] = TA::operand(ta, wm + 32 * i, kk, lane);
+            for (int j = 0; j < NI; ++j) b[kk & 1][j] = TB::operand(tb, wn + 32 * j, kk, lane);
+        };
+        read(0);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) b[j] = TB::operand(tb, wn + 32 * j, kk, lane);
+        for (int kk = 0; kk < KK; ++kk) {
+            if (kk + 1 < KK) read(kk + 1);
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < MI; ++i) {
+                if constexpr (SPREAD) {
+                    if (kk < 2 && k + GF_BK < kend) {
+                        const int p0 = (kk * MI + i) * ALL / SLOTS, p1 = (kk * MI + i + 1) * ALL / SLOTS;
+                        ga.template load<false>(P.a, (u16 *)other, k + GF_BK, kend, min(p0, TA::LOADS), min(p1, TA::LOADS));
+                        gb.template load<EP == EP_GLU>(P.b, (u16 *)other + TA::SIZE, k + GF_BK, kend, max(p0 - TA::LOADS, 0), max(p1 - TA::LOADS, 0));
+                    }
+                }
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = PCM_MFMA16(a[i], b[j], acc[i][j]);
+                for (int j = 0; j < NI; ++j) acc[i][j] = PCM_MFMA16(a[kk & 1][i], b[kk & 1][j], acc[i][j]);
+                if (SPREAD && kk < 2) __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     if (k0 < kend) {
@@ -610,21 +631,23 @@ long gf_tiles(long M, long N, GfShape s) { return (M + s.bm - 1) / s.bm * ((N + 
 
 // The shape of a product's tiles: large ones pass the least data per product through LDS and cache, but a launch of 257 of them takes as long as one
 // of 512.  Taken: the largest shape whose last round of workgroups is not mostly empty (256 compute units, 1 / 2 / 3 workgroups each); over a short
-// contraction the smaller ones, of which one multiplies while its neighbour is in the epilogue.
-GfShape gf_shape(long M, long N, long K, int nsplit)
+// contraction the smaller ones, of which one multiplies while its neighbour is in the epilogue.  Weight gradients, both of whose operands are read
+// transposed, have no registers left for large ones.
+GfShape gf_shape(long M, long N, long K, int nsplit, bool wgrad)
 {
     const long large = gf_tiles(M, N, GF_LARGE) * nsplit, middle = gf_tiles(M, N, GF_MIDDLE) * nsplit;
-    if (K / nsplit >= 1024 && large >= 200 && large * 10 >= (large + 255) / 256 * 256 * 7) return GF_LARGE;
+    if (!wgrad && K / nsplit >= 512 && large >= 200 && large * 10 >= (large + 255) / 256 * 256 * 7) return GF_LARGE;
     return middle >= 256 ? GF_MIDDLE : GF_SMALL;
 }
 
 template <int EP, bool ACOL, bool BCOL>
 void gf_launch(const GfParams &P, hipStream_t s)
 {
-    const GfShape t = gf_shape(P.M, P.N, P.K, P.nsplit);
+    const GfShape t = gf_shape(P.M, P.N, P.K, P.nsplit, EP == EP_WGRAD);
     const dim3 grid((unsigned)((gf_tiles(P.M, P.N, t) * P.nsplit + 7) / 8 * 8));
-    if (t.bm == 256) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 4, 2, 4>), grid, dim3(512), 0, s, P);
-    else if (t.bm == 128) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 2, 2, 2>), grid, dim3(256), 0, s, P);
+    if (t.bm == 256) {
+        if constexpr (EP != EP_WGRAD) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 4, 2, 4>), grid, dim3(512), 0, s, P);
+    } else if (t.bm == 128) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 2, 2, 2>), grid, dim3(256), 0, s, P);
     else hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 1, 2, 2>), grid, dim3(256), 0, s, P);
 }
 
@@ -664,7 +687,7 @@ long gf_back_part_bytes(long R, int E, int F)
 }
 int gf_slots(long R) { return (int)(R < 64 ? 1 : (R / 32 > 512 ? 512 : R / 32)); }
 // partial rows of da | du: two wave rows per tile row
-long gf_wave_rows(long R, int E, long Fp) { const int bm = gf_shape(R, Fp, gf_up(E, 8), 1).bm; return (R + bm - 1) / bm * 2; }
+long gf_wave_rows(long R, int E, long Fp) { const int bm = gf_shape(R, Fp, gf_up(E, 8), 1, false).bm; return (R + bm - 1) / bm * 2; }
 long gf_sum_bytes(long R, int E, long Fp) { return gf_up((gf_wave_rows(R, E, Fp) * 2 * Fp + gf_slots(R) * gf_up(E, 8)) * 4, 256); }
 bool gf_sizes_ok(long R, int E, int F) { return R <= 0x3FFFFFFFL && E <= (1 << 20) && F <= (1 << 20); }
 long gf_pack_bytes(long rows, int cols) { return gf_up(rows * gf_up(cols, 8) * 2, 256); }
