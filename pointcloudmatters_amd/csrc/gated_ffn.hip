@@ -409,9 +409,10 @@ __global__ void __launch_bounds__(256) pcm_gated_close_kernel(GfClose P)
     while (j < P.n && blk >= P.j[j].end) ++j;
     if (j < P.n) {
         const GfJoin &J = P.j[j];
-        const long i = ((blk - (j ? P.j[j - 1].end : 0)) * 256 + threadIdx.x) * 4, size = J.M * J.N;
-        if (i >= size) return;
+        const long first = (blk - (j ? P.j[j - 1].end : 0)) * 1024, size = J.M * J.N;
         if (J.N % 4 == 0) {
+            const long i = first + 4 * (int)threadIdx.x;
+            if (i >= size) return;
             const long row = i / J.N, n = i - row * J.N;
             const bool second = row >= J.osplit;
             const long rr = second ? row - J.osplit : row;
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(256) pcm_gated_close_kernel(GfClose P)
             else o[0] = gf_bf(s.x), o[1] = gf_bf(s.y), o[2] = gf_bf(s.z), o[3] = gf_bf(s.w);
             return;
         }
-        for (long e = i; e < i + 4 && e < size; ++e) {
+        for (long e = first + (int)threadIdx.x; e < first + 1024 && e < size; e += 256) {
             const long row = e / J.N, n = e - row * J.N;
             const bool second = row >= J.osplit;
             const long rr = second ? row - J.osplit : row;

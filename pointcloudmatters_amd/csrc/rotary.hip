@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int ROT_MAX_HALF = 128, ROT_MAX_AXES = 8, ROT_THREADS = 256, ROT_TABLE = 2048;
+constexpr int ROT_MAX_HALF = 128, ROT_MAX_AXES = 8, ROT_THREADS = 256, ROT_TABLE = 2048, ROT_TOKENS = 256;
 
 struct RotArgs {
     const void *x;
@@ -80,13 +80,64 @@ __device__ __forceinline__ float2 rot_cos_sin(double coord, double rev, float si
     return make_float2((k == 1.f || k == 2.f) ? -cc : cc, sign * (k >= 2.f ? -ss : ss));
 }
 
+// One item of the stream: V channels of each half of V pairs; V neighbouring channels, V / 2 pairs, when interleaved (one pair of single
+// channels for V = 1); or V channels behind the pairs.
+template <typename T, int V, bool INTER>
+struct RotItem {
+    typedef Pack<T, V> Vec;
+    static constexpr bool TWO = !INTER || V == 1;   // two accesses
+    static constexpr int PAIRS = TWO ? V : V / 2;
+    Vec a, e;
+    T *o0, *o1;
+    const float2 *cs;  // nullptr: channels that pass through
+    __device__ __forceinline__ void load(const RotArgs &P, const long *xo, const long *oo, const float2 *table, int t, int h, int c, int turned)
+    {
+        const T *x = (const T *)P.x + xo[t] + h * P.x_hs;
+        T *o = (T *)P.out + oo[t] + h * P.o_hs;
+        if (c >= turned) {
+            const int d = 2 * P.half + (c - turned) * V;
+            a = *(const Vec *)(x + d), o0 = o + d, cs = nullptr;
+            return;
+        }
+        const int d0 = INTER ? 2 * c * PAIRS : c * V, d1 = INTER ? d0 + 1 : P.half + c * V;
+        a = *(const Vec *)(x + d0), o0 = o + d0, cs = table + t * P.half + c * PAIRS;
+        if constexpr (TWO) e = *(const Vec *)(x + d1), o1 = o + d1;
+    }
+    __device__ __forceinline__ void finish() const
+    {
+        if (cs == nullptr) {
+            *(Vec *)o0 = a;
+            return;
+        }
+        float u[V], v[V];
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) {
+            const float2 w = cs[j];
+            if constexpr (TWO) {
+                const float p = to_f(a.v[j]), q = to_f(e.v[j]);
+                u[j] = __builtin_fmaf(p, w.x, -(q * w.y)), v[j] = __builtin_fmaf(p, w.y, q * w.x);
+            } else {
+                const float p = to_f(a.v[2 * j]), q = to_f(a.v[2 * j + 1]);
+                u[2 * j] = __builtin_fmaf(p, w.x, -(q * w.y)), u[2 * j + 1] = __builtin_fmaf(p, w.y, q * w.x);
+            }
+        }
+        *(Vec *)o0 = from_f<V>(u, T());
+        if constexpr (TWO) *(Vec *)o1 = from_f<V>(v, T());
+    }
+};
+
 // T: uint16_t (bf16 bits) or float.  V: channels a thread takes from each half of the pairs, one aligned access of V values.
 template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(ROT_THREADS) pcm_rotary_kernel(RotArgs P)
 {
     __shared__ float2 table[ROT_TABLE];  // [token][half]
+    __shared__ long xo[ROT_TOKENS], oo[ROT_TOKENS];
     const long t0 = (long)blockIdx.x * P.tokens;
     const int nt = (int)(P.rows - t0 < P.tokens ? P.rows - t0 : P.tokens);
+    for (int t = threadIdx.x; t < nt; t += ROT_THREADS) {
+        const long b = (t0 + t) / P.L, l = t0 + t - b * P.L;
+        xo[t] = b * P.x_bs + l * P.x_ls, oo[t] = b * P.o_bs + l * P.o_ls;
+    }
     for (int i = threadIdx.x; i < nt * P.half; i += ROT_THREADS) {
         const int t = i / P.half, j = i - t * P.half;
         const long tok = t0 + t, b = tok / P.L;
@@ -97,44 +148,33 @@ __global__ void __launch_bounds__(ROT_THREADS) pcm_rotary_kernel(RotArgs P)
         table[i] = rot_cos_sin(c, P.rev[j], P.sign);
     }
     __syncthreads();
-    const int turned = P.half / V, chunks = turned + (P.D - 2 * P.half) / V, per_token = P.H * chunks;
-    for (int i = threadIdx.x; i < nt * per_token; i += ROT_THREADS) {
-        const int t = i / per_token, r = i - t * per_token, h = r / chunks, c = r - h * chunks;
-        const long tok = t0 + t, b = tok / P.L, l = tok - b * P.L;
-        const T *x = (const T *)P.x + b * P.x_bs + l * P.x_ls + h * P.x_hs;
-        T *o = (T *)P.out + b * P.o_bs + l * P.o_ls + h * P.o_hs;
-        typedef Pack<T, V> Vec;
-        if (c >= turned) {
-            const int d = 2 * P.half + (c - turned) * V;
-            *(Vec *)(o + d) = *(const Vec *)(x + d);
-            continue;
-        }
-        const int d0 = INTER ? 2 * c * V : c * V, d1 = INTER ? d0 + V : P.half + c * V;
-        const Vec a = *(const Vec *)(x + d0), e = *(const Vec *)(x + d1);
-        const float2 *cs = table + t * P.half + c * V;
-        float u[V], v[V];
-        if constexpr (INTER && V == 1) {
-            const float2 w = cs[0];
-            const float p = to_f(a.v[0]), q = to_f(e.v[0]);
-            u[0] = __builtin_fmaf(p, w.x, -(q * w.y)), v[0] = __builtin_fmaf(p, w.y, q * w.x);
-        } else {
+    // items in memory order, (token, head, chunk) carried along instead of divided out; the loads of U items in flight
+    const int turned = P.half / RotItem<T, V, INTER>::PAIRS, chunks = turned + (P.D - 2 * P.half) / V, per_token = P.H * chunks, all = nt * per_token;
+    const int dt = ROT_THREADS / per_token, rest = ROT_THREADS - dt * per_token, dh = rest / chunks, dc = rest - dh * chunks;
+    int t = (int)threadIdx.x / per_token, h = ((int)threadIdx.x - t * per_token) / chunks, c = (int)threadIdx.x - t * per_token - h * chunks;
+    const auto next = [&]() {
+        c += dc;
+        if (c >= chunks) c -= chunks, ++h;
+        h += dh;
+        if (h >= P.H) h -= P.H, ++t;
+        t += dt;
+    };
+    constexpr int U = RotItem<T, V, INTER>::TWO ? 1 : 4;
+    RotItem<T, V, INTER> x[U];
+    int i = threadIdx.x;
+    for (; i + (U - 1) * ROT_THREADS < all; i += U * ROT_THREADS) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float2 w = cs[j];
-                if constexpr (INTER) {  // pair j: channels 2 j, 2 j + 1 of the 2 V channels a | e
-                    const float p = to_f(2 * j < V ? a.v[(2 * j) % V] : e.v[(2 * j) % V]);
-                    const float q = to_f(2 * j + 1 < V ? a.v[(2 * j + 1) % V] : e.v[(2 * j + 1) % V]);
-                    const float f = __builtin_fmaf(p, w.x, -(q * w.y)), g = __builtin_fmaf(p, w.y, q * w.x);
-                    if (2 * j < V) u[(2 * j) % V] = f, u[(2 * j + 1) % V] = g;
-                    else v[(2 * j) % V] = f, v[(2 * j + 1) % V] = g;
-                } else {
-                    const float p = to_f(a.v[j]), q = to_f(e.v[j]);
-                    u[j] = __builtin_fmaf(p, w.x, -(q * w.y)), v[j] = __builtin_fmaf(p, w.y, q * w.x);
-                }
-            }
+        for (int n = 0; n < U; ++n) {
+            x[n].load(P, xo, oo, table, t, h, c, turned);
+            next();
         }
-        *(Vec *)(o + d0) = from_f<V>(u, T());
-        *(Vec *)(o + d1) = from_f<V>(v, T());
+#pragma unroll
+        for (int n = 0; n < U; ++n) x[n].finish();
+    }
+    for (; i < all; i += ROT_THREADS) {
+        x[0].load(P, xo, oo, table, t, h, c, turned);
+        next();
+        x[0].finish();
     }
 }
 
@@ -171,7 +211,7 @@ extern "C" int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, 
     P.x_bs = x_bs, P.x_ls = x_ls, P.x_hs = x_hs, P.o_bs = o_bs, P.o_ls = o_ls, P.o_hs = o_hs, P.c_bs = c_bs, P.c_ls = c_ls;
     P.H = H, P.D = D, P.coords_type = coords_type, P.sign = inverse ? -1.f : 1.f;
     // tokens of a workgroup: as many as the table holds (a long stream per workgroup), fewer while that leaves compute units idle
-    P.tokens = ROT_TABLE / P.half;
+    P.tokens = ROT_TABLE / P.half < ROT_TOKENS ? ROT_TABLE / P.half : ROT_TOKENS;
     while (P.tokens > 1 && P.rows / P.tokens < 1024) P.tokens = (P.tokens + 1) / 2;
     if ((P.rows + P.tokens - 1) / P.tokens > 0x7FFFFFFFL) return PCM_ERR_UNSUPPORTED;
     // the widest access that every channel offset and address is aligned to (16 bytes when strides and sections allow)
