@@ -39,6 +39,11 @@ struct XaParams {
     int tiles, nsplit;
     u16 *out, *dq, *dk, *dv;
     float *lse, *delta, *part_o, *part_ml;
+    // row / G by one multiplication: g_inv = 2^g_shift / G rounded up, 2^(g_shift - 31) >= G.  g_inv * G exceeds 2^g_shift by less than G,
+    // so the product is off by less than row * G <= 2^31 * 2^(g_shift - 31) of 2^g_shift: exact for every row below 2^31
+    uint32_t g_inv;
+    int g_shift;
+    __device__ __forceinline__ int token(int row) const { return (int)(((uint64_t)(uint32_t)row * g_inv) >> g_shift); }
 };
 
 // One side of one sequence: row0 = index of its first row among all rows of the side, n = its rows.
@@ -163,14 +168,14 @@ struct XaStage {
     }
 };
 // rows = token * G + g of a (token, head, channel) matrix
-template <int DP, int ROWS>
-struct XaRowStage : XaStage<DP, ROWS, 256> {
-    typedef XaStage<DP, ROWS, 256> Base;
-    __device__ __forceinline__ void load_rows(const u16 *a, long a_ls, long a_hs, u16 *ta, const u16 *b, long b_ls, long b_hs, u16 *tb, int row0, int n, int G, int wave) const
+template <int DP, int ROWS, int THREADS>
+struct XaRowStage : XaStage<DP, ROWS, THREADS> {
+    typedef XaStage<DP, ROWS, THREADS> Base;
+    __device__ __forceinline__ void load_rows(const u16 *a, long a_ls, long a_hs, u16 *ta, const u16 *b, long b_ls, long b_hs, u16 *tb, int row0, int n, const XaParams &P, int wave) const
     {
 #pragma unroll
         for (int i = 0; i < Base::N; ++i) {
-            const int row = row0 + Base::r + i * Base::NR, tok = G == 1 ? row : row / G, g = row - tok * G;
+            const int row = row0 + Base::r + i * Base::NR, tok = P.token(row), g = row - tok * P.G;
             const int pn = Base::p ^ (8 * xa_swz<DP>(i * Base::NR));
             const bool ok = pn < Base::dim && row < n;
             Base::put(a + tok * a_ls + g * a_hs + pn, ok, ta, i, wave);
@@ -202,17 +207,33 @@ __device__ __forceinline__ void xa_hide(f16v &s, unsigned keys, int h, float v)
 
 // Transposed operand: lane <-> channel 32 * blk + lane % 32, contracted index i of half h <-> tile row row16 + 4 h + i % 4 + 8 (i / 4):
 // the order in which a 32 x 32 accumulator holds 16 of its rows.
+// A lane's two offsets serve every operand of every tile: the permutation is a XOR of the piece with bits of the row, so another piece is
+// a XOR of the offset, and rows a multiple of 16 further are a constant.
 template <int DP>
-__device__ __forceinline__ bf8 xa_transposed(const u16 *tile, int row16, int blk, int lane)
-{
-    const int p = lane & 15, g = (lane >> 4) & 1, h = lane >> 5, r = row16 + 4 * h + (p >> 2), c = 4 * blk + 2 * g + ((p >> 1) & 1);
-    return cat8(xa_tr(tile + xa_at<DP>(r, c) + 4 * (p & 1)), xa_tr(tile + xa_at<DP>(r + 8, c) + 4 * (p & 1)));
-}
-template <int DP>
-__device__ __forceinline__ bf8 xa_rows_operand(const u16 *tile, int row0, int t, int lane)  // lane <-> row, channels 16 t + 8 h ..
-{
-    return lds_bf8(tile + xa_at<DP>(row0 + (lane & 31), 2 * t + (lane >> 5)));
-}
+struct XaLane {
+    int row, tr;
+    __device__ __forceinline__ XaLane(int lane)
+    {
+        const int p = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
+        row = xa_at<DP>(lane & 31, h), tr = xa_at<DP>(4 * h + (p >> 2), 2 * g + ((p >> 1) & 1)) + 4 * (p & 1);
+    }
+    // A copy whose offsets the compiler cannot trace back: it would form all 16 of them in front of a loop and, where registers are short,
+    // read each back from scratch memory; formed at their use they cost one operation.
+    __device__ __forceinline__ XaLane here() const
+    {
+        XaLane c = *this;
+        asm volatile("" : "+v"(c.row), "+v"(c.tr));
+        return c;
+    }
+    __device__ __forceinline__ bf8 rows(const u16 *tile, int row0, int t) const  // lane <-> row, channels 16 t + 8 h ..; row0: a multiple of 32
+    {
+        return lds_bf8(tile + row0 * DP + (row ^ (16 * t)));
+    }
+    __device__ __forceinline__ bf8 transposed(const u16 *tile, int row16, int blk) const  // 8 rows further the permutation's piece bit 1 flips
+    {
+        return cat8(xa_tr(tile + row16 * DP + (tr ^ (32 * blk))), xa_tr(tile + (row16 + 8) * DP + (tr ^ (32 * blk + 16))));
+    }
+};
 
 __device__ __forceinline__ unsigned xa_mask_byte(const unsigned char *m, int key, int n) { return m != nullptr && key < n ? (unsigned)m[key] : 0u; }
 
@@ -283,15 +304,15 @@ struct XaSoftmax {
     }
     // NJ * 32 keys of a tile, c = scale * log2 e
     template <int NJ>
-    __device__ __forceinline__ void tile(const u16 *sk, const u16 *sv, const bf8 (&qf)[DP / 16], unsigned long long vis, float c, int lane)
+    __device__ __forceinline__ void tile(const u16 *sk, const u16 *sv, const bf8 (&qf)[DP / 16], unsigned long long vis, float c, const XaLane<DP> &ln0, int h)
     {
-        const int h = lane >> 5;
+        const XaLane<DP> ln = ln0.here();
         f16v s[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             s[j] = xa_zero16();
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) s[j] = PCM_MFMA16(xa_rows_operand<DP>(sk, 32 * j, t, lane), qf[t], s[j]);
+            for (int t = 0; t < DP / 16; ++t) s[j] = PCM_MFMA16(ln.rows(sk, 32 * j, t), qf[t], s[j]);
         }
         if (vis != (NJ == 2 ? ~0ull : 0xFFFFFFFFull)) {
 #pragma unroll
@@ -324,7 +345,7 @@ struct XaSoftmax {
         for (int t = 0; t < 2 * NJ; ++t) {
             const bf8 p = xa_pack(s[t >> 1], t & 1);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(xa_transposed<DP>(sv, 16 * t, i, lane), p, o[i]);
+            for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(ln.transposed(sv, 16 * t, i), p, o[i]);
         }
     }
 };
@@ -382,6 +403,7 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
 {
     __shared__ __attribute__((aligned(1024))) u16 sk0[XA_TILE * DP], sv0[XA_TILE * DP], sk1[XA_TILE * DP], sv1[XA_TILE * DP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
+    const XaLane<DP> ln(lane);
     XaRows R;
     if (!xa_rows(P, lane, wave, R)) return;
     bf8 qf[DP / 16];
@@ -390,7 +412,7 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
     w.init();
     const float c = P.scale * XA_LOG2E;
     xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, lane, wave,
-                    [&](const u16 *tk, const u16 *tv, unsigned long long vis) { w.template tile<2>(tk, tv, qf, vis, c, lane); });
+                    [&](const u16 *tk, const u16 *tv, unsigned long long vis) { w.template tile<2>(tk, tv, qf, vis, c, ln, h); });
     w.l += __shfl_xor(w.l, 32);
     xa_finish<DP>(P, R, w.o, w.m, w.l, h);
 }
@@ -405,6 +427,7 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
     __shared__ __attribute__((aligned(1024))) u16 t0[4 * 2 * TILE], t1[4 * 2 * TILE];
     __shared__ float sm[4][32], sl[4][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+    const XaLane<DP> ln(lane);
     XaRows R;
     if (!xa_rows(P, lane, 0, R)) return;
     bf8 qf[DP / 16];
@@ -428,7 +451,7 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
         __builtin_amdgcn_wave_barrier();
         vis = next;
         if (key0 + 128 < R.key_hi) request(key0 + 128, nk);
-        if (vis != 0) w.template tile<1>(tk, tk + TILE, qf, vis, c, lane);
+        if (vis != 0) w.template tile<1>(tk, tk + TILE, qf, vis, c, ln, h);
     };
     int key0 = R.key_lo + 32 * wave;
     if (key0 < R.key_hi) {
@@ -511,6 +534,7 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
 {
     __shared__ __attribute__((aligned(1024))) u16 sk0[XA_TILE * DP], sv0[XA_TILE * DP], sk1[XA_TILE * DP], sv1[XA_TILE * DP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
+    const XaLane<DP> ln0(lane);
     XaRows R;
     if (!xa_rows(P, lane, wave, R)) return;
     bf8 qf[DP / 16], gf[DP / 16];
@@ -534,13 +558,14 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = xa_zero16();
     xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, lane, wave, [&](const u16 *tk, const u16 *tv, unsigned long long vis) {
+        const XaLane<DP> ln = ln0.here();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             f16v s = xa_zero16(), dp = xa_zero16();
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
-                s = PCM_MFMA16(xa_rows_operand<DP>(tk, 32 * j, t, lane), qf[t], s);
-                dp = PCM_MFMA16(xa_rows_operand<DP>(tv, 32 * j, t, lane), gf[t], dp);
+                s = PCM_MFMA16(ln.rows(tk, 32 * j, t), qf[t], s);
+                dp = PCM_MFMA16(ln.rows(tv, 32 * j, t), gf[t], dp);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -552,7 +577,7 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
             for (int u = 0; u < 2; ++u) {
                 const bf8 ds = xa_pack(s, u);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(xa_transposed<DP>(tk, 32 * j + 16 * u, i, lane), ds, o[i]);
+                for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(ln.transposed(tk, 32 * j + 16 * u, i), ds, o[i]);
             }
         }
     });
@@ -579,102 +604,261 @@ __global__ void __launch_bounds__(256) pcm_xattn_dq_join_kernel(XaParams P)
     *(uint2 *)(P.dq + 4 * i) = make_uint2(cvt_pk_bf16(a.x * P.scale, a.y * P.scale), cvt_pk_bf16(a.z * P.scale, a.w * P.scale));
 }
 
-template <int DP>
-__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) pcm_xattn_dkv_kernel(XaParams P)
+// What a key kernel's workgroup works on: 128 keys of a (sequence, key head), and a share of its rows.
+struct XaKeys {
+    int b, kvh, split, key0, lo, nrows;  // rows lo .. nrows - 1
+    XaSpan qs, ks;
+    long kb, kr;  // batch and first row of the sequence in K and V
+    const unsigned char *mask;
+};
+__device__ __forceinline__ bool xa_keys(const XaParams &P, int lane, XaKeys &K)
 {
-    __shared__ __attribute__((aligned(1024))) u16 sq0[XA_TILE * DP], sg0[XA_TILE * DP], sq1[XA_TILE * DP], sg1[XA_TILE * DP];
+    const long items = (long)P.tiles * P.Hkv * P.nsplit, item = xa_item(items);
+    if (item >= items) return false;
+    int tile;
+    const long rest = item / P.tiles;
+    K.kvh = (int)(rest % P.Hkv), K.split = (int)(rest / P.Hkv);
+    if (!xa_locate(P.kv_off, P.B, P.S, P.kv_rows, 1, XA_ROWS, (int)(item % P.tiles), lane, K.b, tile)) return false;
+    K.ks = xa_span(P.kv_off, K.b, P.B, P.S, P.kv_rows);
+    K.qs = K.b < P.B ? xa_span(P.q_off, K.b, P.B, P.L, P.q_rows) : XaSpan{0, 0};
+    K.key0 = tile * XA_ROWS;
+    const int all = K.qs.n * P.G, rt = (all + XA_TILE - 1) / XA_TILE, per = (rt + P.nsplit - 1) / P.nsplit * XA_TILE;
+    K.lo = K.split * per, K.nrows = min(all, K.lo + per);
+    K.kb = P.kv_off ? 0 : (long)K.b, K.kr = P.kv_off ? K.ks.row0 : 0;
+    K.mask = P.mask ? P.mask + (P.kv_off ? K.ks.row0 : K.kb * P.mask_bs) : nullptr;
+    return true;
+}
+
+// The rows of a key kernel, 64 at a time through two LDS buffers of Q and dO and of the rows' statistics.
+template <int DP, int THREADS>
+struct XaRowLoop {
+    static constexpr int PIECES = DP / 8, ROWT = XA_TILE * PIECES < THREADS ? XA_TILE * PIECES : THREADS;  // threads that request a tile
+    const XaParams &P;
+    const XaKeys &K;
+    const int wave;
+    XaRowStage<DP, XA_TILE, ROWT> st;
+    const u16 *qb, *gb;
+    float rl, rd;
+    __device__ __forceinline__ XaRowLoop(const XaParams &P_, const XaKeys &K_, int wave_) : P(P_), K(K_), wave(wave_), qb(nullptr), gb(nullptr)
+    {
+        st.init((int)threadIdx.x, P.D);
+        if (K.lo >= K.nrows) return;
+        qb = P.q + (P.q_off ? K.qs.row0 * P.q_ls : K.b * P.q_bs) + (long)K.kvh * P.G * P.q_hs;
+        gb = P.dout + (P.q_off ? K.qs.row0 * P.g_ls : K.b * P.g_bs) + (long)K.kvh * P.G * P.g_hs;
+    }
+    __device__ __forceinline__ void request(int row0, u16 *tq, u16 *tg)
+    {
+        // the statistics first, untouched until they are stored: waiting for them then leaves the tiles behind them in flight
+        const int row = row0 + (int)threadIdx.x, tok = P.token(row);
+        rl = -INFINITY, rd = 0.f;
+        if (threadIdx.x < XA_TILE && row < K.nrows) {
+            const long at = (K.qs.row0 + tok) * P.H + K.kvh * P.G + (row - tok * P.G);
+            rl = P.lse[at], rd = P.delta[at];
+        }
+        if (ROWT == THREADS || wave < ROWT / 64) st.load_rows(qb, P.q_ls, P.q_hs, tq, gb, P.g_ls, P.g_hs, tg, row0, K.nrows, P, wave);
+    }
+    template <class F>
+    __device__ __forceinline__ void step(int row0, int buf, const u16 *tq, const u16 *tg, u16 *nq, u16 *ng, float (*sl)[XA_TILE], float (*sd)[XA_TILE], F &body)
+    {
+        if (threadIdx.x < XA_TILE) sl[buf][threadIdx.x] = rl == -INFINITY ? INFINITY : rl * XA_LOG2E, sd[buf][threadIdx.x] = rd;
+        xa_arrived();
+        if (row0 + XA_TILE < K.nrows) request(row0 + XA_TILE, nq, ng);
+        body(buf, tq, tg);
+    }
+    template <class F>
+    __device__ __forceinline__ void run(u16 *sq0, u16 *sg0, u16 *sq1, u16 *sg1, float (*sl)[XA_TILE], float (*sd)[XA_TILE], F &body)
+    {
+        if (K.lo >= K.nrows) return;
+        request(K.lo, sq0, sg0);
+        int row0 = K.lo;
+        for (; row0 + XA_TILE < K.nrows; row0 += 2 * XA_TILE) {
+            step(row0, 0, sq0, sg0, sq1, sg1, sl, sd, body);
+            step(row0 + XA_TILE, 1, sq1, sg1, sq0, sg0, sl, sd, body);
+        }
+        if (row0 < K.nrows) step(row0, 0, sq0, sg0, sq1, sg1, sl, sd, body);
+    }
+};
+// s := P, dp := dS of a 32 x 32 tile (a lane's key, 16 rows in its registers)
+__device__ __forceinline__ void xa_weights(f16v &s, f16v &dp, const float *sl, const float *sd, float c, bool seen, int h)
+{
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const float4 l2 = *(const float4 *)(sl + 8 * g + 4 * h), de = *(const float4 *)(sd + 8 * g + 4 * h);
+        const float a[4] = {l2.x, l2.y, l2.z, l2.w}, e[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * g + i;
+            const float p = seen ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -a[i])) : 0.f;
+            dp[r] = p * (dp[r] - e[i]), s[r] = p;
+        }
+    }
+}
+template <int DP>
+__device__ __forceinline__ void xa_store_keys(const XaParams &P, const XaKeys &K, int key, int h, const f16v (&dk)[DP / 32], const f16v (&dv)[DP / 32])
+{
+    const long at = ((K.ks.row0 + key) * P.Hkv + K.kvh) * P.D, whole = P.kv_rows * P.Hkv * P.D;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        if (P.nsplit > 1) {
+            xa_store_part(P.part_o + 2 * K.split * whole + at, P.D, h, i, dk[i]);
+            xa_store_part(P.part_o + (2 * K.split + 1) * whole + at, P.D, h, i, dv[i]);
+        } else {
+            xa_store_row(P.dk + at, P.D, h, i, dk[i], P.scale);
+            xa_store_row(P.dv + at, P.D, h, i, dv[i], 1.f);
+        }
+    }
+}
+
+// dK and dV of 128 keys, heads wider than 64.  8 waves: four groups of 32 keys times the two halves of every 64-row tile of Q and dO, whose sums
+// are added at the end.  K and V stand in LDS beside the two buffers of Q and dO (128 KB): held in registers, as operands of 4 waves,
+// they left one wave a SIMD, which waited for its own LDS reads and exponentials (515 x 4 rows over 1027 keys: 119 us, now 88).
+// nsplit > 1: the rows are shared out and each share writes fp32 sums.
+template <int DP>
+__global__ void __launch_bounds__(512, 2) pcm_xattn_dkv_wide_kernel(XaParams P)
+{
+    __shared__ __attribute__((aligned(1024))) u16 sq0[XA_TILE * DP], sg0[XA_TILE * DP], sq1[XA_TILE * DP], sg1[XA_TILE * DP], sk[XA_ROWS * DP],
+        sv[XA_ROWS * DP];
     __shared__ __attribute__((aligned(16))) float sl[2][XA_TILE], sd[2][XA_TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-    const long items = (long)P.tiles * P.Hkv, item = xa_item(items);
-    if (item >= items) return;
-    int b, tile;
-    const int kvh = (int)(item / P.tiles);
-    if (!xa_locate(P.kv_off, P.B, P.S, P.kv_rows, 1, XA_ROWS, (int)(item % P.tiles), lane, b, tile)) return;
-    const XaSpan ks = xa_span(P.kv_off, b, P.B, P.S, P.kv_rows);
-    const XaSpan qs = b < P.B ? xa_span(P.q_off, b, P.B, P.L, P.q_rows) : XaSpan{0, 0};
-    const int key = tile * XA_ROWS + wave * 32 + col, nrows = qs.n * P.G;
-    const bool held = key < ks.n;
-    const long key_row = ks.row0 + key, kb = P.kv_off ? 0 : (long)b, kr = P.kv_off ? key_row : (long)key;
-    const bool seen = held && (P.mask == nullptr || P.mask[P.kv_off ? key_row : kb * P.mask_bs + key] == 0);
-    bf8 kf[DP / 16], vf[DP / 16];
-    xa_row_operand<DP>(P.k + kb * P.k_bs + kr * P.k_ls + (long)kvh * P.k_hs, seen, P.D, h, kf);
-    xa_row_operand<DP>(P.v + kb * P.v_bs + kr * P.v_ls + (long)kvh * P.v_hs, seen, P.D, h, vf);
-    const u16 *qb = nrows == 0 ? nullptr : P.q + (P.q_off ? qs.row0 * P.q_ls : b * P.q_bs) + (long)kvh * P.G * P.q_hs;
-    const u16 *gb = nrows == 0 ? nullptr : P.dout + (P.q_off ? qs.row0 * P.g_ls : b * P.g_bs) + (long)kvh * P.G * P.g_hs;
+    const XaLane<DP> ln0(lane);
+    const int kg = wave & 3, half = wave >> 2;
+    XaKeys K;
+    if (!xa_keys(P, lane, K)) return;
+    const int key = K.key0 + kg * 32 + col;
+    const bool held = key < K.ks.n, seen = held && (K.mask == nullptr || K.mask[key] == 0);
     const float c = P.scale * XA_LOG2E;
     f16v dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = xa_zero16(), dv[i] = xa_zero16();
-    XaRowStage<DP, XA_TILE> st;
-    st.init((int)threadIdx.x, P.D);
-    float rl = -INFINITY, rd = 0.f;
-    const auto request = [&](int row0, u16 *tq, u16 *tg) {
-        // the statistics first, untouched until they are stored: waiting for them then leaves the tiles behind them in flight
-        const int row = row0 + (int)threadIdx.x, tok = row / P.G;
-        rl = -INFINITY, rd = 0.f;
-        if (threadIdx.x < XA_TILE && row < nrows) {
-            const long at = (qs.row0 + tok) * P.H + kvh * P.G + (row - tok * P.G);
-            rl = P.lse[at], rd = P.delta[at];
+    if (K.lo < K.nrows) {  // K and V, zeros for keys that are not there or not seen
+        XaStage<DP, XA_ROWS, 512> kt;
+        kt.init((int)threadIdx.x, P.D);
+        const u16 *kp = P.k + K.kb * P.k_bs + K.kr * P.k_ls + (long)K.kvh * P.k_hs, *vp = P.v + K.kb * P.v_bs + K.kr * P.v_ls + (long)K.kvh * P.v_hs;
+#pragma unroll
+        for (int n = 0; n < kt.N; ++n) {
+            const int j = K.key0 + kt.r + n * kt.NR, pn = kt.p ^ (8 * xa_swz<DP>(n * kt.NR));
+            const bool ok = pn < P.D && j < K.ks.n && (K.mask == nullptr || K.mask[j] == 0);
+            kt.put(kp + (long)j * P.k_ls + pn, ok, sk, n, wave), kt.put(vp + (long)j * P.v_ls + pn, ok, sv, n, wave);
         }
-        st.load_rows(qb, P.q_ls, P.q_hs, tq, gb, P.g_ls, P.g_hs, tg, row0, nrows, P.G, wave);
+    }
+    XaRowLoop<DP, 512> rows(P, K, wave);
+    const auto body = [&](int buf, const u16 *tq, const u16 *tg) {
+        const XaLane<DP> ln = ln0.here();
+        f16v s = xa_zero16(), dp = xa_zero16();
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            s = PCM_MFMA16(ln.rows(tq, 32 * half, t), ln.rows(sk, 32 * kg, t), s);
+            dp = PCM_MFMA16(ln.rows(tg, 32 * half, t), ln.rows(sv, 32 * kg, t), dp);
+        }
+        xa_weights(s, dp, sl[buf] + 32 * half, sd[buf] + 32 * half, c, seen, h);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bf8 p = xa_pack(s, u), ds = xa_pack(dp, u);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                dv[i] = PCM_MFMA16(ln.transposed(tg, 32 * half + 16 * u, i), p, dv[i]);
+                dk[i] = PCM_MFMA16(ln.transposed(tq, 32 * half + 16 * u, i), ds, dk[i]);
+            }
+        }
     };
-    const auto step = [&](int row0, int buf, const u16 *tq, const u16 *tg, u16 *nq, u16 *ng) {
-        if (threadIdx.x < XA_TILE) sl[buf][threadIdx.x] = rl == -INFINITY ? INFINITY : rl * XA_LOG2E, sd[buf][threadIdx.x] = rd;
-        xa_arrived();
-        if (row0 + XA_TILE < nrows) request(row0 + XA_TILE, nq, ng);
+    rows.run(sq0, sg0, sq1, sg1, sl, sd, body);
+    // the two halves: [register][lane], dK and then dV, 128 * DP values in the place of K and V
+    float *const sum = (float *)(kg < 2 ? sk : sv) + (kg & 1) * 32 * DP;
+    __syncthreads();
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        if (half == 1) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[(16 * i + r) * 64 + lane] = part ? dv[i][r] : dk[i][r];
+        }
+        __syncthreads();
+        if (half == 0) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float v = sum[(16 * i + r) * 64 + lane];
+                    if (part) dv[i][r] += v;
+                    else dk[i][r] += v;
+                }
+        }
+        __syncthreads();
+    }
+    if (half == 0 && held) xa_store_keys<DP>(P, K, key, h, dk, dv);
+}
+
+// The same for heads of up to 64: 4 waves, K and V of a wave's 32 keys in registers, both halves of a row tile one after the other.
+template <int DP>
+__global__ void __launch_bounds__(256, 2) pcm_xattn_dkv_narrow_kernel(XaParams P)
+{
+    __shared__ __attribute__((aligned(1024))) u16 sq0[XA_TILE * DP], sg0[XA_TILE * DP], sq1[XA_TILE * DP], sg1[XA_TILE * DP];
+    __shared__ __attribute__((aligned(16))) float sl[2][XA_TILE], sd[2][XA_TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+    const XaLane<DP> ln0(lane);
+    XaKeys K;
+    if (!xa_keys(P, lane, K)) return;
+    const int key = K.key0 + wave * 32 + col;
+    const bool held = key < K.ks.n, seen = held && (K.mask == nullptr || K.mask[key] == 0);
+    const long at_k = K.kb * P.k_bs + (K.kr + key) * P.k_ls + (long)K.kvh * P.k_hs, at_v = K.kb * P.v_bs + (K.kr + key) * P.v_ls + (long)K.kvh * P.v_hs;
+    bf8 kf[DP / 16], vf[DP / 16];
+    xa_row_operand<DP>(P.k + (seen ? at_k : 0), seen, P.D, h, kf);
+    xa_row_operand<DP>(P.v + (seen ? at_v : 0), seen, P.D, h, vf);
+    const float c = P.scale * XA_LOG2E;
+    f16v dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) dk[i] = xa_zero16(), dv[i] = xa_zero16();
+    XaRowLoop<DP, 256> rows(P, K, wave);
+    const auto body = [&](int buf, const u16 *tq, const u16 *tg) {
+        const XaLane<DP> ln = ln0.here();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             f16v s = xa_zero16(), dp = xa_zero16();
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
-                s = PCM_MFMA16(xa_rows_operand<DP>(tq, 32 * j, t, lane), kf[t], s);
-                dp = PCM_MFMA16(xa_rows_operand<DP>(tg, 32 * j, t, lane), vf[t], dp);
+                s = PCM_MFMA16(ln.rows(tq, 32 * j, t), kf[t], s);
+                dp = PCM_MFMA16(ln.rows(tg, 32 * j, t), vf[t], dp);
             }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 l2 = *(const float4 *)(sl[buf] + 32 * j + 8 * g + 4 * h), de = *(const float4 *)(sd[buf] + 32 * j + 8 * g + 4 * h);
-                const float a[4] = {l2.x, l2.y, l2.z, l2.w}, e[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 4 * g + i;
-                    const float p = seen ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -a[i])) : 0.f;
-                    dp[r] = p * (dp[r] - e[i]), s[r] = p;
-                }
-            }
+            xa_weights(s, dp, sl[buf] + 32 * j, sd[buf] + 32 * j, c, seen, h);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const bf8 p = xa_pack(s, u), ds = xa_pack(dp, u);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) {
-                    dv[i] = PCM_MFMA16(xa_transposed<DP>(tg, 32 * j + 16 * u, i, lane), p, dv[i]);
-                    dk[i] = PCM_MFMA16(xa_transposed<DP>(tq, 32 * j + 16 * u, i, lane), ds, dk[i]);
+                    dv[i] = PCM_MFMA16(ln.transposed(tg, 32 * j + 16 * u, i), p, dv[i]);
+                    dk[i] = PCM_MFMA16(ln.transposed(tq, 32 * j + 16 * u, i), ds, dk[i]);
                 }
             }
         }
     };
-    if (nrows > 0) {
-        request(0, sq0, sg0);
-        int row0 = 0;
-        for (; row0 + XA_TILE < nrows; row0 += 2 * XA_TILE) {
-            step(row0, 0, sq0, sg0, sq1, sg1);
-            step(row0 + XA_TILE, 1, sq1, sg1, sq0, sg0);
-        }
-        if (row0 < nrows) step(row0, 0, sq0, sg0, sq1, sg1);
-    }
-    if (!held) return;
-    const long at = (key_row * P.Hkv + kvh) * P.D;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-        xa_store_row(P.dk + at, P.D, h, i, dk[i], P.scale);
-        xa_store_row(P.dv + at, P.D, h, i, dv[i], 1.f);
-    }
+    rows.run(sq0, sg0, sq1, sg1, sl, sd, body);
+    if (held) xa_store_keys<DP>(P, K, key, h, dk, dv);
 }
 
-#define XA_BY_DIM(kernel, grid, s, P)                                                                       \
+// dK and dV out of the shares of their rows, in order: four channels a thread, dK then dV
+__global__ void __launch_bounds__(256) pcm_xattn_dkv_join_kernel(XaParams P)
+{
+    const long quads = P.kv_rows * P.Hkv * (P.D / 4);
+    long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= 2 * quads) return;
+    const int part = i >= quads;
+    i -= part * quads;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < P.nsplit; ++s) {
+        const float4 v = *(const float4 *)(P.part_o + 4 * ((2 * s + part) * quads + i));
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+    const float f = part ? 1.f : P.scale;
+    *(uint2 *)((part ? P.dv : P.dk) + 4 * i) = make_uint2(cvt_pk_bf16(a.x * f, a.y * f), cvt_pk_bf16(a.z * f, a.w * f));
+}
+
+#define XA_BY_DIM(kernel, threads, grid, s, P)                                                              \
     do {                                                                                                    \
-        if ((P).D <= 32) hipLaunchKernelGGL((kernel<32>), dim3(grid), dim3(256), 0, s, P);                  \
-        else if ((P).D <= 64) hipLaunchKernelGGL((kernel<64>), dim3(grid), dim3(256), 0, s, P);             \
-        else hipLaunchKernelGGL((kernel<128>), dim3(grid), dim3(256), 0, s, P);                             \
+        if ((P).D <= 32) hipLaunchKernelGGL((kernel<32>), dim3(grid), dim3(threads), 0, s, P);              \
+        else if ((P).D <= 64) hipLaunchKernelGGL((kernel<64>), dim3(grid), dim3(threads), 0, s, P);         \
+        else hipLaunchKernelGGL((kernel<128>), dim3(grid), dim3(threads), 0, s, P);                         \
     } while (0)
 
 bool xa_shape_ok(int H, int Hkv, int D) { return H > 0 && Hkv > 0 && H % Hkv == 0 && D >= 8 && D <= 128 && D % 8 == 0; }
@@ -692,17 +876,30 @@ bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows
 // Splits of the keys.  A workgroup per (tile, key head) is too few for 256 compute units when the rows are few (one token of a rollout,
 // a decoder's 100 queries): the keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and
 // re-reads its row's fp32 sums and costs a second launch (4 - 5 us), so it has 256 keys at least (for one row over 2051 keys, 8 heads: 10 us
-// with 8 splits, 20 with one).
+// with 8 splits, 20 with one).  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave
+// hides the others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 255 us with one split, 192 + 10
+// for the joining with four).
 int xa_splits(int B, int H, int Hkv, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed)
 {
     const int G = H / Hkv;
     const long work = (q_packed ? (q_rows * G + XA_ROWS - 1) / XA_ROWS + B - 1 : xa_tiles(0, B, L, q_rows, G, XA_ROWS)) * Hkv;
-    const long keys = kv_packed ? (kv_rows + B - 1) / B : S, least = 256;
-    long n = 512 / (work > 0 ? work : 1);
-    n = n < keys / least ? n : keys / least;
+    const long keys = kv_packed ? (kv_rows + B - 1) / B : S, w = work > 0 ? work : 1;
+    long n = 512 / w < keys / 256 ? 512 / w : keys / 256;
+    const long more = 1536 / w < keys / 2048 ? 1536 / w : keys / 2048;
+    n = n > more ? n : more;
     return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
 int xa_splits(const XaParams &P) { return xa_splits(P.B, P.H, P.Hkv, P.L, P.q_rows, P.q_off != nullptr, P.S, P.kv_rows, P.kv_off != nullptr); }
+
+// Splits of the rows for dK and dV, where few keys leave compute units idle: at least 512 rows (8 tiles) each.
+int xa_row_splits(int B, int Hkv, int G, long q_rows, int S, long kv_rows, int kv_packed)
+{
+    const long work = (kv_packed ? (kv_rows + XA_ROWS - 1) / XA_ROWS + B - 1 : xa_tiles(0, B, S, kv_rows, 1, XA_ROWS)) * Hkv;
+    const long rows = q_rows * G / B, w = work > 0 ? work : 1;
+    const long n = 256 / w < rows / 512 ? 256 / w : rows / 512;
+    return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
+}
+int xa_row_splits(const XaParams &P) { return xa_row_splits(P.B, P.Hkv, P.G, P.q_rows, P.S, P.kv_rows, P.kv_off != nullptr); }
 
 bool xa_strides_ok(const void *p, long bs, long ls, long hs) { return (((uintptr_t)p) & 15) == 0 && ((bs | ls | hs) & 7) == 0; }
 
@@ -715,13 +912,16 @@ int xa_fill(XaParams &P, int B, int H, int Hkv, int D, int L, long q_rows, const
     if (!(scale > 0.f) || scale > 3.0e38f) return PCM_ERR_BAD_ARG;
     if (!q_offset) q_rows = (long)B * L;
     if (!kv_offset) kv_rows = (long)B * S;
-    if (q_rows * H > 0x7FFFFFFFL || kv_rows > 0x7FFFFFFFL || (kv_rows + 127) / 128 * Hkv + (long)B * Hkv > 0x3FFFFFFFL) return PCM_ERR_UNSUPPORTED;
+    if (q_rows * H > 0x7FFFFF00L || kv_rows > 0x7FFFFF00L || (kv_rows + 127) / 128 * Hkv + (long)B * Hkv > 0x3FFFFFFFL) return PCM_ERR_UNSUPPORTED;
     if ((q_rows > 0 && !q) || (kv_rows > 0 && (!k || !v))) return PCM_ERR_BAD_ARG;
     if (!xa_strides_ok(q, q_bs, q_ls, q_hs) || !xa_strides_ok(k, k_bs, k_ls, k_hs) || !xa_strides_ok(v, v_bs, v_ls, v_hs)) return PCM_ERR_UNSUPPORTED;
     P.q = (const u16 *)q, P.k = (const u16 *)k, P.v = (const u16 *)v;
     P.q_bs = q_bs, P.q_ls = q_ls, P.q_hs = q_hs, P.k_bs = k_bs, P.k_ls = k_ls, P.k_hs = k_hs, P.v_bs = v_bs, P.v_ls = v_ls, P.v_hs = v_hs;
     P.mask = mask, P.mask_bs = mask_bs, P.q_off = q_offset, P.kv_off = kv_offset;
     P.B = B, P.H = H, P.Hkv = Hkv, P.G = H / Hkv, P.D = D, P.L = L, P.S = S, P.q_rows = q_rows, P.kv_rows = kv_rows, P.scale = scale;
+    P.g_shift = 31;
+    while ((1L << (P.g_shift - 31)) < P.G) ++P.g_shift;
+    P.g_inv = (uint32_t)(((1ull << P.g_shift) + P.G - 1) / P.G);
     return PCM_OK;
 }
 
@@ -735,8 +935,10 @@ extern "C" long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, lon
 {
     if (B <= 0 || L < 0 || S < 0 || q_rows < 0 || kv_rows < 0 || !xa_shape_ok(H, Hkv, D)) return 0;
     if (!q_packed) q_rows = (long)B * L;
-    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed);
-    return n > 1 ? (long)n * q_rows * H * (D + 2) * 4 : 0;
+    if (!kv_packed) kv_rows = (long)B * S;
+    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed), m = xa_row_splits(B, Hkv, H / Hkv, q_rows, S, kv_rows, kv_packed);
+    const long rows = n > 1 ? (long)n * q_rows * H * (D + 2) * 4 : 0, keys = m > 1 ? (long)m * 2 * kv_rows * Hkv * D * 4 : 0;
+    return rows > keys ? rows : keys;
 }
 
 extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
@@ -760,8 +962,8 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     }
     P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS);
     const hipStream_t s = (hipStream_t)stream;
-    if (few) XA_BY_DIM(pcm_xattn_few_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
-    else XA_BY_DIM(pcm_xattn_fwd_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
+    if (few) XA_BY_DIM(pcm_xattn_few_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
+    else XA_BY_DIM(pcm_xattn_fwd_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
     if (P.nsplit > 1) {
         const long rows = P.q_rows * H;
         if (D <= 32) hipLaunchKernelGGL((pcm_xattn_join_kernel<8>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, P);
@@ -797,12 +999,21 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
             P.part_o = (float *)ws;
         }
         P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS);
-        XA_BY_DIM(pcm_xattn_dq_kernel, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
+        XA_BY_DIM(pcm_xattn_dq_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
         if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_dq_join_kernel, dim3((unsigned)((P.q_rows * H * (D / 4) + 255) / 256)), dim3(256), 0, s, P);
     }
     if (P.kv_rows > 0) {
         P.tiles = (int)xa_tiles(kv_offset != nullptr, B, S, P.kv_rows, 1, XA_ROWS);
-        XA_BY_DIM(pcm_xattn_dkv_kernel, xa_grid((long)P.tiles * Hkv), s, P);
+        P.nsplit = xa_row_splits(P);
+        if (P.nsplit > 1) {
+            if (!ws || ws_bytes < (long)P.nsplit * 2 * P.kv_rows * Hkv * D * 4) return PCM_ERR_BAD_ARG;
+            P.part_o = (float *)ws;
+        }
+        const dim3 grid(xa_grid((long)P.tiles * Hkv * P.nsplit));
+        if (D <= 32) hipLaunchKernelGGL((pcm_xattn_dkv_narrow_kernel<32>), grid, dim3(256), 0, s, P);
+        else if (D <= 64) hipLaunchKernelGGL((pcm_xattn_dkv_narrow_kernel<64>), grid, dim3(256), 0, s, P);
+        else hipLaunchKernelGGL((pcm_xattn_dkv_wide_kernel<128>), grid, dim3(512), 0, s, P);
+        if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_dkv_join_kernel, dim3((unsigned)((P.kv_rows * Hkv * (D / 2) + 255) / 256)), dim3(256), 0, s, P);
     }
     return PCM_LAUNCH_STATUS();
 }
