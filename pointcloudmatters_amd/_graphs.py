@@ -105,16 +105,20 @@ def captured(fn, pool=None):
 
 
 def guard_leaves(out, what):
-    """`out`, the result of an autograd function whose inputs may be leaves -- refused during a capture when an eager graph over the
-    same leaves is alive.  autograd keeps ONE accumulation node per leaf, for as long as any graph holds it, on the stream it was made
-    on; a backward pass captured on another stream then draws that stream into the capture, and ending the capture ends the process
-    (a segmentation fault inside the runtime).  Eager calls note their stream on the node; a captured call that finds another one
-    raises instead.  Freeing the eager graph (its outputs) frees the node."""
+    """`out`, the result of an autograd function whose inputs may be leaves, views of them or casts -- refused during a capture when an
+    eager graph over the same leaves is alive.  autograd keeps ONE accumulation node per leaf, for as long as any graph holds it, on the
+    stream it was made on; a backward pass captured on another stream then draws that stream into the capture, and ending the capture
+    ends the process (a segmentation fault inside the runtime).  Eager calls note their stream on the node; a captured call that finds
+    another one raises instead.  Freeing the eager graph (its outputs) frees the node."""
     if out.grad_fn is None:
         return out
     here, capturing = _lib.raw_stream(), torch.cuda.is_current_stream_capturing()
     for node, _ in out.grad_fn.next_functions:
-        if node is not None and node.name().endswith("AccumulateGrad"):
+        for _ in range(4):  # through what a wrapper puts in front: a view, a cast, a copy
+            if node is None or len(node.next_functions) != 1:
+                break
+            node = node.next_functions[0][0]
+        if node is not None and not node.next_functions and node.name().endswith("AccumulateGrad"):
             made = node.metadata.setdefault("pcm_stream", here)
             if capturing and made != here:
                 raise RuntimeError("%s: an eager graph over the same leaf tensors is alive: free its outputs before a backward pass "

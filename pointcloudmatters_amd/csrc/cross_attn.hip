@@ -912,7 +912,12 @@ int xa_fill(XaParams &P, int B, int H, int Hkv, int D, int L, long q_rows, const
     if (!(scale > 0.f) || scale > 3.0e38f) return PCM_ERR_BAD_ARG;
     if (!q_offset) q_rows = (long)B * L;
     if (!kv_offset) kv_rows = (long)B * S;
-    if (q_rows * H > 0x7FFFFF00L || kv_rows > 0x7FFFFF00L || (kv_rows + 127) / 128 * Hkv + (long)B * Hkv > 0x3FFFFFFFL) return PCM_ERR_UNSUPPORTED;
+    // rows and keys are 32-bit numbers inside a sequence, with room for the steps that pass its end; a launch has fewer than 2^32 threads
+    // (splits only multiply launches of a few hundred workgroups)
+    if (q_rows > 0x7FFFFC00L / H || kv_rows > 0x7FFFFC00L) return PCM_ERR_UNSUPPORTED;
+    if (xa_tiles(q_offset != nullptr, B, L, q_rows, H / Hkv, XA_ROWS) > 0xFFFFF000L / 256 / Hkv ||
+        xa_tiles(kv_offset != nullptr, B, S, kv_rows, 1, XA_ROWS) > 0xFFFFF000L / 512 / Hkv)
+        return PCM_ERR_UNSUPPORTED;
     if ((q_rows > 0 && !q) || (kv_rows > 0 && (!k || !v))) return PCM_ERR_BAD_ARG;
     if (!xa_strides_ok(q, q_bs, q_ls, q_hs) || !xa_strides_ok(k, k_bs, k_ls, k_hs) || !xa_strides_ok(v, v_bs, v_ls, v_hs)) return PCM_ERR_UNSUPPORTED;
     P.q = (const u16 *)q, P.k = (const u16 *)k, P.v = (const u16 *)v;

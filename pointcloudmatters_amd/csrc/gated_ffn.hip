@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(128 * WN, 2) pcm_gated_gemm_kernel(GfParams P)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = slab[r * SLAB + c + e];
             if constexpr (EP == EP_GLU) {
+                if (col >= P.Fp) continue;  // a tile of 256 columns, 128 of each projection, may end behind the last of 64 k
                 float u[8], hv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) u[e] = slab[r * SLAB + 32 + c + e];
@@ -690,7 +691,11 @@ int gf_slots(long R) { return (int)(R < 64 ? 1 : (R / 32 > 512 ? 512 : R / 32));
 // partial rows of da | du: two wave rows per tile row
 long gf_wave_rows(long R, int E, long Fp) { const int bm = gf_shape(R, Fp, gf_up(E, 8), 1, false).bm; return (R + bm - 1) / bm * 2; }
 long gf_sum_bytes(long R, int E, long Fp) { return gf_up((gf_wave_rows(R, E, Fp) * 2 * Fp + gf_slots(R) * gf_up(E, 8)) * 4, 256); }
-bool gf_sizes_ok(long R, int E, int F) { return R <= 0x3FFFFFFFL && E <= (1 << 20) && F <= (1 << 20); }
+// 32-bit rows and columns inside a tile; no launch has 2^32 threads (a copy of x, dy and three weights takes one for eight values)
+bool gf_sizes_ok(long R, int E, int F)
+{
+    return R <= 0x3FFFFFFFL && E <= (1 << 20) && F <= (1 << 20) && R * gf_up(E, 8) <= 1L << 33 && R * gf_up(F, 64) <= 1L << 36 && (long)F * E <= 1L << 32;
+}
 long gf_pack_bytes(long rows, int cols) { return gf_up(rows * gf_up(cols, 8) * 2, 256); }
 
 }  // namespace

@@ -195,7 +195,8 @@ extern "C" int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, 
     if (B < 0 || L < 0 || H < 0 || D < 0 || axes < 0) return PCM_ERR_BAD_ARG;
     if (B == 0 || L == 0 || H == 0 || D == 0) return PCM_OK;
     if (!x || !out || !coords || !sections || axes < 1 || axes > ROT_MAX_AXES || coords_type < 0 || coords_type > 2) return PCM_ERR_BAD_ARG;
-    if (!(base > 0.0) || L > (1L << 40) / B || (long)H * D > (1L << 24)) return PCM_ERR_BAD_ARG;
+    if (!(base > 0.0)) return PCM_ERR_BAD_ARG;
+    if (L > (1L << 40) / B || (long)H * D > (1L << 22)) return PCM_ERR_UNSUPPORTED;  // a workgroup's items are a 32-bit number
     RotArgs P;
     P.half = 0;
     for (int a = 0; a < axes; ++a) {
@@ -213,7 +214,7 @@ extern "C" int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, 
     // tokens of a workgroup: as many as the table holds (a long stream per workgroup), fewer while that leaves compute units idle
     P.tokens = ROT_TABLE / P.half < ROT_TOKENS ? ROT_TABLE / P.half : ROT_TOKENS;
     while (P.tokens > 1 && P.rows / P.tokens < 1024) P.tokens = (P.tokens + 1) / 2;
-    if ((P.rows + P.tokens - 1) / P.tokens > 0x7FFFFFFFL) return PCM_ERR_UNSUPPORTED;
+    if ((P.rows + P.tokens - 1) / P.tokens > 0xFFFFFFL) return PCM_ERR_UNSUPPORTED;  // fewer than 2^32 threads
     // the widest access that every channel offset and address is aligned to (16 bytes when strides and sections allow)
     const int size = x_is_bf16 ? 2 : 4;
     int V = 16 / size;

@@ -46,16 +46,17 @@ def _launch(x, coords, sections, base, interleaved, inverse):
 
 class _RotaryAxes(Function):
     @staticmethod
-    def forward(ctx, x, coords, sections, base, interleaved):
+    def forward(ctx, x, coords, sections, base, interleaved, inverse):
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(coords)
-            ctx.meta = (sections, base, interleaved)
-        return _launch(x, coords, sections, base, interleaved, False)
+            ctx.meta = (sections, base, interleaved, not inverse)
+        return _launch(x, coords, sections, base, interleaved, inverse)
 
     @staticmethod
     def backward(ctx, dout):
         (coords,) = ctx.saved_tensors
-        return _launch(dout, coords, *ctx.meta, True), None, None, None, None
+        turn = _RotaryAxes.apply if torch.is_grad_enabled() and dout.requires_grad else _launch  # linear: its own backward, turned back
+        return turn(dout, coords, *ctx.meta), None, None, None, None, None
 
 
 def rotary_axes(x, coords, sections, base=10000.0, interleaved=False):
@@ -90,4 +91,4 @@ def rotary_axes(x, coords, sections, base=10000.0, interleaved=False):
         coords = coords.contiguous()
     if not (torch.is_grad_enabled() and x.requires_grad):
         return _launch(x, coords, sections, float(base), bool(interleaved), False)
-    return _graphs.guard_leaves(_RotaryAxes.apply(x, coords, sections, float(base), bool(interleaved)), "rotary_axes")
+    return _graphs.guard_leaves(_RotaryAxes.apply(x, coords, sections, float(base), bool(interleaved), False), "rotary_axes")

@@ -206,3 +206,29 @@ def test_runs_repeat_bit_for_bit():
     args = _inputs((2, 70), (2, 900), 2, 64, 4, seed=18)
     a, b = _run(*args, None, None, None), _run(*args, None, None, None)
     assert torch.equal(a[0], b[0]) and all(torch.equal(x, y) for x, y in zip(a[2], b[2]))
+
+
+@pytest.mark.parametrize("b,l,s,heads,hkv,d", [(1, 16, 70, 4, 2, 64), (1, 17, 70, 4, 2, 64), (1, 32, 150, 1, 1, 128), (2, 33, 150, 2, 2, 32), (1, 30, 50, 7, 1, 32),
+                                               (1, 9, 70, 24, 1, 8), (2, 11, 66, 13, 1, 104)])
+def test_rows_of_a_key_head_around_a_tile(b, l, s, heads, hkv, d):
+    """16 x 2, 32 x 1 rows: one 32-row tile; more: several.  Groups of 7, 13 and 24 heads: rows divided by what is no power of two."""
+    _check(*_inputs((b, l), (b, s), hkv, d, heads, seed=21), None, None, None)
+
+
+def test_few_packed_rows():
+    _check(*_inputs((16,), (214,), 2, 64, 4, seed=22), None, [3, 0, 13], [100, 50, 64])
+
+
+@pytest.mark.parametrize("b,l,s,heads,hkv,d", [(1, 1200, 40, 4, 2, 64), (2, 1100, 70, 2, 1, 128), (1, 1500, 20, 1, 1, 32)])
+def test_rows_shared_out_over_workgroups(b, l, s, heads, hkv, d):
+    """Few keys under many rows: the dK and dV sums of the row ranges are joined."""
+    mask = torch.zeros(b, s, dtype=torch.bool)
+    mask[0, 3:17] = True
+    _check(*_inputs((b, l), (b, s), hkv, d, heads, seed=23), mask, None, None)
+
+
+def test_long_states_under_many_rows_at_size():
+    """Packed sides of several thousand rows and keys: the rule that shares long states out further."""
+    mask = torch.zeros(8300, dtype=torch.bool)
+    mask[100:2400] = True
+    _check(*_inputs((4700,), (8300,), 4, 16, 8, seed=24), mask, [2300, 2400], [4200, 4100])

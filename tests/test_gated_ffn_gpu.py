@@ -131,3 +131,27 @@ def test_runs_repeat_bit_for_bit():
     args = _inputs(1500, 64, 100, True, seed=7)
     a, b = _run(*args, "silu"), _run(*args, "silu")
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("r", [2, 3, 8, 9])
+def test_few_rows_and_one_more(r):
+    _check(_inputs(r, 72, 100, True, seed=8), "silu")
+
+
+@pytest.mark.parametrize("r,e,f", [(8200, 520, 1700), (8200, 1544, 520)])
+def test_large_tiles_at_size(r, e, f):
+    """Products of over 200 tiles of 256 x 256, the last of them ragged in rows and columns and half outside the hidden columns."""
+    _check(_inputs(r, e, f, True, seed=9), "silu")
+
+
+def test_weights_of_different_alignment():
+    """Gate and up weights as parts of one buffer, the second not at a 16-byte boundary."""
+    from pointcloudmatters_amd.policy import gated_ffn
+
+    x, wg, wu, wd, bg, bu, bd, _ = _inputs(40, 48, 72, True, seed=10)
+    want = gated_ffn(*(t.to(DEV) for t in (x, wg, wu, wd, bg, bu, bd)))
+    for start in (0, 1):
+        buf = torch.zeros(start + 2 * wg.numel() + 3, dtype=torch.bfloat16, device=DEV)
+        g, u = buf[start:start + wg.numel()].view_as(wg), buf[start + wg.numel() + 3:][:wu.numel()].view_as(wu)
+        g.copy_(wg), u.copy_(wu)
+        assert torch.equal(gated_ffn(x.to(DEV), g, u, *(t.to(DEV) for t in (wd, bg, bu, bd))), want)

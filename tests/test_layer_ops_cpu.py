@@ -13,7 +13,7 @@ from tests.wavesim import build as _build
 needs_model = pytest.mark.skipif(not os.path.exists(_build.CLANG), reason="needs the ROCm clang++ as host compiler (tests/wavesim)")
 
 GPU_FILES = ("test_rotary_gpu", "test_cross_attn_gpu", "test_gated_ffn_gpu", "test_layer_ops_gpu")
-NEEDS_HIP_RUNTIME = ("stream", "captur")
+NEEDS_HIP_RUNTIME = ("stream", "captur", "at_size")  # at_size: too long for the model
 
 
 def _adopt():
@@ -139,6 +139,8 @@ def test_entry_points_reject_before_they_touch_the_runtime():
     assert rot(D=14) == 1 and rot(axes=9) == 1 and rot(axes=0) == 1 and rot(base=0.0) == 1 and rot(ct=3) == 1 and rot(x=None) == 1
     assert rot(sec=(ctypes.c_int * 2)(100, 100), D=512) == 2 and rot(sec=(ctypes.c_int * 2)(-1, 4)) == 2 and rot(sec=(ctypes.c_int * 2)(0, 0)) == 1
 
+    assert rot(D=1 << 22) == 2
+
     def xa(H=2, Hkv=1, D=64, q=p, q_ls=128, scale=1.0, out=p, ws=None, wsb=0, S=5, kv_rows=5, back=False):
         head = (1, H, Hkv, D, 3, 3, None, S, kv_rows, None, q, 0, q_ls, 64, p, 0, 64, 64, p, 0, 64, 64, None, 0, scale)
         if back:
@@ -149,6 +151,7 @@ def test_entry_points_reject_before_they_touch_the_runtime():
         assert xa(H=3, Hkv=2, back=back) == 2 and xa(D=60, back=back) == 2 and xa(D=136, back=back) == 2 and xa(q_ls=129, back=back) == 2
         assert xa(q=0x1008, back=back) == 2 and xa(q=None, back=back) == 1 and xa(scale=0.0, back=back) == 1 and xa(out=None, back=back) == 1
         assert xa(scale=float("nan"), back=back) == 1
+        assert xa(S=0x7FFFFF00, back=back) == 2 and xa(H=1 << 10, Hkv=1 << 10, S=0x7FFFF000, back=back) == 2  # more threads than a launch takes
         assert xa(S=100000, back=back) == 1  # split keys need their workspace
     assert L.pcm_cross_attn_supported(8, 2, 64) == 1 and L.pcm_cross_attn_supported(8, 3, 64) == 0 and L.pcm_cross_attn_supported(8, 2, 4) == 0
     assert L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 5, 5, 0) == 0 < L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 100000, 100000, 0)
@@ -158,7 +161,7 @@ def test_entry_points_reject_before_they_touch_the_runtime():
 
     assert ff(act=3) == 1 and ff(act=-1) == 1 and ff(x=None) == 1 and ff(a=p) == 1 and ff(h=None) == 1 and ff(h=0x1002) == 1 and ff(E=0) == 1
     assert ff(F=7, ws=None, wsb=0) == 1  # an odd width needs its padded copies
-    assert ff(E=1 << 21) == 2
+    assert ff(E=1 << 21) == 2 and ff(R=1 << 30) == 2 and ff(E=1 << 17, F=1 << 17) == 2
     fb = lambda wsb, dwu=p: L.pcm_gated_ffn_backward_hip(4, 16, 8, 0, p, 16, p, p, p, p, p, p, p, 16, p, p, dwu, p, None, None, None, p, wsb, None)  # noqa: E731
     need = L.pcm_gated_ffn_ws_bytes(4, 16, 8, 1)
     assert need > 0 and fb(need - 1) == 1 and fb(need, None) == 1

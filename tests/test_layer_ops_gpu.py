@@ -134,6 +134,33 @@ def test_a_captured_call_is_refused_while_an_eager_graph_of_its_leaves_lives():
     assert all(o.isfinite().all() for o in outs)
 
 
+def test_a_captured_call_sees_the_leaves_behind_casts_and_views():
+    from pointcloudmatters_amd import _graphs
+    from pointcloudmatters_amd.policy import cross_attention, gated_ffn
+
+    x, wg, wu, wd = (torch.randn(*s).to(DEV).requires_grad_() for s in ((4, 16), (24, 16), (24, 16), (16, 24)))
+    q, k = torch.randn(1, 3, 64).bfloat16().to(DEV).requires_grad_(), torch.randn(1, 9, 64).bfloat16().to(DEV).requires_grad_()
+
+    def cast():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return gated_ffn(x, wg, wu, wd)
+
+    calls = [cast, lambda: cross_attention(*(t.unflatten(-1, (2, 32)) for t in (q, k, k)))]
+    alive = [f() for f in calls]
+
+    def refused():
+        for f in calls:
+            with pytest.raises(RuntimeError, match="eager graph"):
+                f()
+        return x.detach() + 1
+
+    graph, _ = _graphs.captured(refused)
+    graph.replay()
+    torch.cuda.synchronize()
+    for t in alive:
+        t.sum().backward()
+
+
 def test_two_captured_graphs_share_nothing():
     """Two graphs with workspaces of their own (split keys, padded copies), replayed one inside the other's work."""
     from pointcloudmatters_amd import _graphs
