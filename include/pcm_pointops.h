@@ -703,8 +703,8 @@ int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, long q_rows
 
 /* ---- gated feed-forward block (csrc/gated_ffn.hip) ------------------------------------------------------------------
  * y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd; bf16; x (R, E) at row stride x_ls, wg / wu (F, E), wd (E, F) contiguous, biases
- * nullable; act 0 SiLU, 1 GELU (erf), 2 ReLU; any E and F.  y (R, E) contiguous.  h (R, Fp) and, for a backward pass, a, u (R, Fp; both or
- * neither): the hidden values and the two projections at Fp = pcm_gated_ffn_hidden_ld(F) values a row, 16-byte aligned.
+ * nullable; act 0 SiLU, 1 GELU (erf), 2 ReLU; any E and F.  y (R, E) contiguous.  h (R, Fp) and, for a backward pass, a, u (R, Fp) fp32,
+ * both or neither: the hidden values and the two projections at Fp = pcm_gated_ffn_hidden_ld(F) values a row, 16-byte aligned.
  * Backward: gradients that are NULL are not computed (dwg with dwu, dbg with dbu).  ws: pcm_gated_ffn_ws_bytes bytes (0: none), 16-byte aligned.
  * No atomics: results are reproducible. */
 long pcm_gated_ffn_hidden_ld(int F);

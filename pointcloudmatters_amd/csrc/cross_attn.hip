@@ -18,7 +18,8 @@
 //
 // Masked or absent keys are zeroed in K and V where a tile is staged (a NaN or infinity in padding must not meet a zero weight) and
 // their scores are replaced by -inf.  Sums, maxima, lse, delta and accumulators are fp32; P and dS are rounded to bf16 (one half step,
-// 2^-8 relative at most) because the matrix operands are bf16; outputs are rounded once.
+// 2^-8 relative at most) because the matrix operands are bf16; outputs are rounded once; delta reads O as it was stored (its rounding's
+// part of dQ is a fraction of dS's own: O is an average of V).
 #include "pcm_attn.hpp"
 
 namespace {

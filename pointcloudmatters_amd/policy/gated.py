@@ -29,7 +29,7 @@ def _empty(n, dev):
 
 
 def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
-    """y, and for a backward pass (keep) the hidden tensors a | u | h in one buffer, else None."""
+    """y, and for a backward pass (keep) the hidden tensors a | u (fp32) | h in one buffer, else None."""
     L_ = _lib.load()
     (rows, e), f, dev = x.shape, w_gate.shape[0], x.device
     with _lib.on_device(dev):
@@ -37,9 +37,9 @@ def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
         n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, False)
         y = torch.empty((rows, e), dtype=x.dtype, device=dev)
         size = 2 * rows * ld
-        hidden = _empty(3 * size if keep else size + n, dev)  # without a backward pass: h, then the workspace
+        hidden = _empty(5 * size if keep else size + n, dev)  # without a backward pass: h, then the workspace
         p = hidden.data_ptr()
-        a, u, h = (p, p + size, p + 2 * size) if keep else (0, 0, p)
+        a, u, h = (p, p + 2 * size, p + 4 * size) if keep else (0, 0, p)
         ws = _empty(n, dev) if keep and n else None
         rc = L_.pcm_gated_ffn_forward_hip(rows, e, f, act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                                           _ptr(b_gate), _ptr(b_up), _ptr(b_down), y.data_ptr(), a, u, h, _ptr(ws) if keep else p + size, n,
@@ -74,9 +74,9 @@ class _GatedFFN(Function):
             dbd = new((e,), dtype=dtype, device=dev) if need[6] else None
             n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, True)
             ws = _empty(n, dev)
-            p, size = hidden.data_ptr(), hidden.numel() // 3
+            p, size = hidden.data_ptr(), hidden.numel() // 5
             rc = L_.pcm_gated_ffn_backward_hip(rows, e, f, ctx.act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
-                                               w_down.data_ptr(), p, p + size, p + 2 * size, dy.data_ptr(), dy.stride(0), _ptr(dx), _ptr(dwg),
+                                               w_down.data_ptr(), p, p + 2 * size, p + 4 * size, dy.data_ptr(), dy.stride(0), _ptr(dx), _ptr(dwg),
                                                _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), ws.data_ptr(), n, _raw_stream())
         if rc:
             _lib.check(rc, "pcm_gated_ffn_backward_hip")

@@ -136,7 +136,7 @@ def ffn(x, wg, wu, wd, bg, bu, bd, kind, dy=None):
     dh = g @ wd
     edh = (E + 4) * F32 * (g.abs() @ wd.abs())
     da, du = dh * u * ds, dh * s
-    # a and u are read as they were stored
+    # a and u as bf16 at worst (kept in fp32 they are closer)
     sa, su = ea + HALF * (a.abs() + ea), eu + HALF * (u.abs() + eu)
     eds = m2 * sa + 16 * F32 * (1 + a.abs())
     if kind == "relu":
