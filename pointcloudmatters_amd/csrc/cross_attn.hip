@@ -37,7 +37,7 @@ struct XaParams {
     int B, H, Hkv, G, D, L, S;
     long q_rows, kv_rows;
     float scale;
-    int tiles, nsplit;
+    int tiles, each, nsplit;  // each: tiles of a padded sequence
     u16 *out, *dq, *dk, *dv;
     float *lse, *delta, *part_o, *part_ml;
     // row / G by one multiplication: g_inv = 2^g_shift / G rounded up, 2^(g_shift - 31) >= G.  g_inv * G exceeds 2^g_shift by less than G,
@@ -89,11 +89,14 @@ __device__ __forceinline__ bool xa_locate(const int *off, int B, int len, long r
     return false;
 }
 
-// consecutive work items (the tiles of one key head, which read the same K and V) go to one XCD's contiguous share
-__device__ __forceinline__ long xa_item(long items)
+// Consecutive work items (the tiles of one key head, which read the same K and V) go to one XCD's contiguous share.  Padded sides: where a
+// share is whole runs of `each` tiles, the runs' first tiles are started first and their last ones, which are ragged, at the end.
+__device__ __forceinline__ long xa_item(long items, int each)
 {
-    const long per = (items + 7) / 8;
-    return (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const int per = (int)((items + 7) / 8), x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    if (each <= 1 || per % each != 0) return (long)x * per + i;
+    const int runs = per / each, tile = i / runs;
+    return (long)x * per + (long)(i - tile * runs) * each + tile;
 }
 
 typedef s4 __attribute__((address_space(3))) * xa_lds_s4;
@@ -258,7 +261,7 @@ __device__ __forceinline__ void xa_store_part(float *row, int D, int h, int blk,
 // What a row kernel's workgroup works on.
 struct XaRows {
     int b, kvh, split, row, tok, head, nrows, key_lo, key_hi;  // key range: multiples of XA_TILE
-    bool ok;
+    bool ok, work;  // the lane's row is there; a row of the wave is
     XaSpan qs, ks;
     const u16 *k, *v;
     const unsigned char *mask;
@@ -266,7 +269,7 @@ struct XaRows {
 };
 __device__ __forceinline__ bool xa_rows(const XaParams &P, int lane, int wave, XaRows &R)
 {
-    const long items = (long)P.tiles * P.Hkv * P.nsplit, item = xa_item(items);
+    const long items = (long)P.tiles * P.Hkv * P.nsplit, item = xa_item(items, P.each);
     if (item >= items) return false;
     int tile;
     const long rest = item / P.tiles;
@@ -281,6 +284,7 @@ __device__ __forceinline__ bool xa_rows(const XaParams &P, int lane, int wave, X
     const int kt = (R.ks.n + XA_TILE - 1) / XA_TILE, per = (kt + P.nsplit - 1) / P.nsplit;
     R.key_lo = R.split * per * XA_TILE, R.key_hi = min(R.ks.n, R.key_lo + per * XA_TILE);
     const long kb = P.kv_off ? 0 : (long)R.b, kr = P.kv_off ? R.ks.row0 : 0;
+    R.work = __ballot(R.ok) != 0;
     if (R.ks.n == 0) return true;
     R.k = P.k + kb * P.k_bs + kr * P.k_ls + (long)R.kvh * P.k_hs;
     R.v = P.v + kb * P.v_bs + kr * P.v_ls + (long)R.kvh * P.v_hs;
@@ -388,7 +392,7 @@ __device__ __forceinline__ void xa_key_loop(const XaRows &R, const XaParams &P, 
         xa_arrived();
         const unsigned long long vis = next;
         if (key0 + XA_TILE < R.key_hi) request(key0 + XA_TILE, nk, nv);
-        if (vis != 0) body(tk, tv, vis);
+        if (vis != 0 && R.work) body(tk, tv, vis);
     };
     request(R.key_lo, sk0, sv0);
     int key0 = R.key_lo;
@@ -614,7 +618,7 @@ struct XaKeys {
 };
 __device__ __forceinline__ bool xa_keys(const XaParams &P, int lane, XaKeys &K)
 {
-    const long items = (long)P.tiles * P.Hkv * P.nsplit, item = xa_item(items);
+    const long items = (long)P.tiles * P.Hkv * P.nsplit, item = xa_item(items, P.each);
     if (item >= items) return false;
     int tile;
     const long rest = item / P.tiles;
@@ -627,6 +631,10 @@ __device__ __forceinline__ bool xa_keys(const XaParams &P, int lane, XaKeys &K)
     K.lo = K.split * per, K.nrows = min(all, K.lo + per);
     K.kb = P.kv_off ? 0 : (long)K.b, K.kr = P.kv_off ? K.ks.row0 : 0;
     K.mask = P.mask ? P.mask + (P.kv_off ? K.ks.row0 : K.kb * P.mask_bs) : nullptr;
+    if (K.mask != nullptr) {  // keys that are all masked (padding): no rows to go through
+        const int k0 = K.key0 + lane, k1 = k0 + 64;
+        if (__ballot((k0 < K.ks.n && K.mask[k0] == 0) || (k1 < K.ks.n && K.mask[k1] == 0)) == 0) K.nrows = K.lo;
+    }
     return true;
 }
 
@@ -743,7 +751,9 @@ __global__ void __launch_bounds__(512, 2) pcm_xattn_dkv_wide_kernel(XaParams P)
         }
     }
     XaRowLoop<DP, 512> rows(P, K, wave);
+    const bool work = __ballot(seen) != 0;  // a wave whose keys are absent or masked only takes part in the loading
     const auto body = [&](int buf, const u16 *tq, const u16 *tg) {
+        if (!work) return;
         const XaLane<DP> ln = ln0.here();
         f16v s = xa_zero16(), dp = xa_zero16();
 #pragma unroll
@@ -811,7 +821,9 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dkv_narrow_kernel(XaParams P
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = xa_zero16(), dv[i] = xa_zero16();
     XaRowLoop<DP, 256> rows(P, K, wave);
+    const bool work = __ballot(seen) != 0;
     const auto body = [&](int buf, const u16 *tq, const u16 *tg) {
+        if (!work) return;
         const XaLane<DP> ln = ln0.here();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -966,7 +978,7 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
         if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * (D + 2) * 4) return PCM_ERR_BAD_ARG;
         P.part_o = (float *)ws, P.part_ml = (float *)ws + (long)P.nsplit * P.q_rows * H * D;
     }
-    P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS);
+    P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS), P.each = q_offset ? 1 : P.tiles / B;
     const hipStream_t s = (hipStream_t)stream;
     if (few) XA_BY_DIM(pcm_xattn_few_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
     else XA_BY_DIM(pcm_xattn_fwd_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
@@ -1004,12 +1016,12 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
             if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * D * 4) return PCM_ERR_BAD_ARG;
             P.part_o = (float *)ws;
         }
-        P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS);
+        P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS), P.each = q_offset ? 1 : P.tiles / B;
         XA_BY_DIM(pcm_xattn_dq_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
         if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_dq_join_kernel, dim3((unsigned)((P.q_rows * H * (D / 4) + 255) / 256)), dim3(256), 0, s, P);
     }
     if (P.kv_rows > 0) {
-        P.tiles = (int)xa_tiles(kv_offset != nullptr, B, S, P.kv_rows, 1, XA_ROWS);
+        P.tiles = (int)xa_tiles(kv_offset != nullptr, B, S, P.kv_rows, 1, XA_ROWS), P.each = kv_offset ? 1 : P.tiles / B;
         P.nsplit = xa_row_splits(P);
         if (P.nsplit > 1) {
             if (!ws || ws_bytes < (long)P.nsplit * 2 * P.kv_rows * Hkv * D * 4) return PCM_ERR_BAD_ARG;
