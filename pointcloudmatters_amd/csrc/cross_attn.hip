@@ -81,7 +81,7 @@ __device__ __forceinline__ bool xa_locate(const int *off, int B, int len, long r
         const unsigned long long past = __ballot(run + incl > t);
         if (past != 0) {
             const int f = __ffsll(past) - 1;
-            b = base + f, tile = (int)(t - run) - (__shfl(incl, f) - __shfl(mine, f));
+            b = base + f, tile = __builtin_amdgcn_readfirstlane((int)(t - run) - (__shfl(incl, f) - __shfl(mine, f)));
             return true;
         }
         run += __shfl(incl, 63);
@@ -127,6 +127,12 @@ __device__ __forceinline__ void xa_row_operand(const u16 *row, bool ok, int D, i
 __device__ uint4 xa_zeros;
 typedef __attribute__((address_space(3))) void *xa_lds_p;
 typedef const __attribute__((address_space(1))) void *xa_glb_p;
+typedef const __attribute__((address_space(1))) char *xa_glb_c;
+__device__ __forceinline__ const u16 *xa_uniform(const u16 *p)  // the same in all lanes: to scalar registers
+{
+    const uint64_t a = (uint64_t)p;
+    return (const u16 *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)a));
+}
 
 // 64 banks of 4 bytes.  ds_read_b128 serves the lanes 0-3, 12-15, 20-23, 24-27 of 32 together, then the other 16: the rows of either set
 // that share a place modulo 256 bytes must hold a piece in different slots.  ds_read_b64_tr_b16 serves 32 lanes together, 64 bytes of
@@ -142,6 +148,8 @@ __device__ __forceinline__ int xa_at(int row, int piece)  // value offset of a p
 {
     return row * DP + ((piece ^ xa_swz<DP>(row)) << 3);
 }
+
+constexpr long XA_NEAR = 1 << 23;  // 64 rows at smaller strides are less than 2^31 bytes apart
 
 // THREADS threads (a workgroup or one wave) request ROWS rows; a thread's n-th piece stands n * NR rows below its first.
 template <int DP, int ROWS, int THREADS>
@@ -159,9 +167,21 @@ struct XaStage {
     {
         __builtin_amdgcn_global_load_lds((xa_glb_p)(ok ? (const void *)src : (const void *)&xa_zeros), (xa_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, 0, 0);
     }
+    // All rows from `src` on at stride ls < XA_NEAR are wanted, all DP channels: one 32-bit offset a lane beside uniform addresses, and no
+    // selection.  With the general form below, addresses were a fifth of the row kernels' vector instructions.
+    __device__ __forceinline__ void load_all(const u16 *src, int ls, u16 *tile, int wave) const
+    {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const unsigned at = 2u * (unsigned)(r * ls + (p ^ (8 * xa_swz<DP>(n * NR))));
+            const xa_glb_c row = (xa_glb_c)(const char *)xa_uniform(src + (long)(n * NR) * ls);
+            __builtin_amdgcn_global_load_lds((xa_glb_p)(row + at), (xa_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, 0, 0);
+        }
+    }
     // rows row0 .. of a matrix at row stride ls; visible: bit i <-> tile row i
     __device__ __forceinline__ void load(const u16 *base, long ls, long row0, unsigned long long visible, u16 *tile, int wave) const
     {
+        if (visible == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1) && dim == DP && ls < XA_NEAR) return load_all(base + row0 * ls, (int)ls, tile, wave);
         const u16 *src = base + (row0 + r) * ls;
         const unsigned long long mine = visible >> r;
 #pragma unroll
@@ -177,6 +197,12 @@ struct XaRowStage : XaStage<DP, ROWS, THREADS> {
     typedef XaStage<DP, ROWS, THREADS> Base;
     __device__ __forceinline__ void load_rows(const u16 *a, long a_ls, long a_hs, u16 *ta, const u16 *b, long b_ls, long b_hs, u16 *tb, int row0, int n, const XaParams &P, int wave) const
     {
+        // one head a key head, or all of them: rows at one stride
+        const long as = P.G == 1 ? a_ls : a_hs, bs = P.G == 1 ? b_ls : b_hs;
+        if (row0 + ROWS <= n && Base::dim == DP && (P.G == 1 || (a_ls == P.G * a_hs && b_ls == P.G * b_hs)) && as < XA_NEAR && bs < XA_NEAR) {
+            Base::load_all(a + row0 * as, (int)as, ta, wave), Base::load_all(b + row0 * bs, (int)bs, tb, wave);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < Base::N; ++i) {
             const int row = row0 + Base::r + i * Base::NR, tok = P.token(row), g = row - tok * P.G;
@@ -296,7 +322,11 @@ __device__ __forceinline__ const u16 *xa_q_row(const XaParams &P, const u16 *bas
     return base + (P.q_off ? (R.qs.row0 + R.tok) * ls : R.b * bs + R.tok * ls) + (long)R.head * hs;
 }
 
-// One 32-row column of the forward pass: running maximum m and sum l (of this lane's half of the keys) and O^T.
+// One 32-row column of the forward pass: reference m, sum l (of this lane's half of the keys) and O^T.
+// m is a score that the row has met, at least its maximum less XA_SLACK / c: moving it with every new maximum would multiply O^T nearly each
+// tile (32 rows, of which one has a new maximum more often than not) and exchange the halves' maxima; weights up to 2^8 are as good, the sums
+// are fp32 and the bf16 of a weight has the same relative step everywhere.
+constexpr float XA_SLACK = 8.f;
 template <int DP>
 struct XaSoftmax {
     f16v o[DP / 32];
@@ -328,15 +358,15 @@ struct XaSoftmax {
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) mx = max3f(mx, s[j][r], s[j][r + 1]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mc = mx == -INFINITY ? 0.f : mx * c;
-        if (__ballot(mx > m) != 0) {  // a row's maximum has grown: after the first tiles a rare case
-            const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, c, -mc));
+        if (__ballot((mx - m) * c > XA_SLACK) != 0) {  // the first tile; then a rare case
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float alpha = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mx) * c);
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+            m = mx;
         }
-        m = mx;
+        const float mc = m == -INFINITY ? 0.f : m * c;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
