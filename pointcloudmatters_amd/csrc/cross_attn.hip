@@ -265,6 +265,30 @@ struct XaLane {
     }
 };
 
+// LDS reads and matrix instructions keep their order here (vector operations may pass).  The compiler reads an operand right in front of its
+// use and waits out the whole LDS latency each time; with one or two waves a SIMD that was most of the time of a tile.
+__device__ __forceinline__ void xa_keep() { __builtin_amdgcn_sched_barrier(0x406); }
+
+// acc[j] += A_j B_j over the DP channels, for N products: the operands of the next 16 channels are read before the present ones are multiplied
+template <int DP, int N, class FA, class FB>
+__device__ __forceinline__ void xa_products(f16v (&acc)[N], FA a, FB b)
+{
+    bf8 x[2][N], y[2][N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[0][j] = a(j, 0), y[0][j] = b(j, 0);
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        if (t + 1 < DP / 16) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[(t + 1) & 1][j] = a(j, t + 1), y[(t + 1) & 1][j] = b(j, t + 1);
+        }
+        xa_keep();
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = PCM_MFMA16(x[t & 1][j], y[t & 1][j], acc[j]);
+        xa_keep();
+    }
+}
+
 __device__ __forceinline__ unsigned xa_mask_byte(const unsigned char *m, int key, int n) { return m != nullptr && key < n ? (unsigned)m[key] : 0u; }
 
 __device__ __forceinline__ void xa_store_row(u16 *row, int D, int h, int blk, const f16v &o, float f)
@@ -344,11 +368,12 @@ struct XaSoftmax {
         const XaLane<DP> ln = ln0.here();
         f16v s[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            s[j] = xa_zero16();
+        for (int j = 0; j < NJ; ++j) s[j] = xa_zero16();
+        xa_products<DP>(s, [&](int j, int t) { return ln.rows(sk, 32 * j, t); }, [&](int, int t) { return qf[t]; });
+        bf8 vt[2][DP / 32];
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) s[j] = PCM_MFMA16(ln.rows(sk, 32 * j, t), qf[t], s[j]);
-        }
+        for (int i = 0; i < DP / 32; ++i) vt[0][i] = ln.transposed(sv, 0, i);
+        xa_keep();
         if (vis != (NJ == 2 ? ~0ull : 0xFFFFFFFFull)) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) xa_hide(s[j], (unsigned)(vis >> (32 * j)), h, -INFINITY);
@@ -378,9 +403,15 @@ struct XaSoftmax {
         l += sum;
 #pragma unroll
         for (int t = 0; t < 2 * NJ; ++t) {
-            const bf8 p = xa_pack(s[t >> 1], t & 1);
+            if (t + 1 < 2 * NJ) {
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(ln.transposed(sv, 16 * t, i), p, o[i]);
+                for (int i = 0; i < DP / 32; ++i) vt[(t + 1) & 1][i] = ln.transposed(sv, 16 * (t + 1), i);
+            }
+            const bf8 p = xa_pack(s[t >> 1], t & 1);
+            xa_keep();
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(vt[t & 1][i], p, o[i]);
+            xa_keep();
         }
     }
 };
@@ -596,23 +627,29 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
         const XaLane<DP> ln = ln0.here();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f16v s = xa_zero16(), dp = xa_zero16();
+            f16v s[2] = {xa_zero16(), xa_zero16()};  // scores, dP
+            xa_products<DP>(s, [&](int n, int t) { return ln.rows(n ? tv : tk, 32 * j, t); }, [&](int n, int t) { return n ? gf[t] : qf[t]; });
+            bf8 kt[2][DP / 32];
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) {
-                s = PCM_MFMA16(ln.rows(tk, 32 * j, t), qf[t], s);
-                dp = PCM_MFMA16(ln.rows(tv, 32 * j, t), gf[t], dp);
-            }
+            for (int i = 0; i < DP / 32; ++i) kt[0][i] = ln.transposed(tk, 32 * j, i);
+            xa_keep();
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -l2));
-                s[r] = p * (dp[r] - delta);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c, -l2));
+                s[0][r] = p * (s[1][r] - delta);
             }
-            if (vis != ~0ull) xa_hide(s, (unsigned)(vis >> (32 * j)), h, 0.f);
+            if (vis != ~0ull) xa_hide(s[0], (unsigned)(vis >> (32 * j)), h, 0.f);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const bf8 ds = xa_pack(s, u);
+                if (u == 0) {
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(ln.transposed(tk, 32 * j + 16 * u, i), ds, o[i]);
+                    for (int i = 0; i < DP / 32; ++i) kt[1][i] = ln.transposed(tk, 32 * j + 16, i);
+                }
+                const bf8 ds = xa_pack(s[0], u);
+                xa_keep();
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(kt[u][i], ds, o[i]);
+                xa_keep();
             }
         }
     });
@@ -732,6 +769,27 @@ __device__ __forceinline__ void xa_weights(f16v &s, f16v &dp, const float *sl, c
         }
     }
 }
+// dV += dO^T P, dK += Q^T dS over 32 rows of a tile
+template <int DP>
+__device__ __forceinline__ void xa_key_products(f16v (&dk)[DP / 32], f16v (&dv)[DP / 32], const f16v &p, const f16v &ds, const XaLane<DP> &ln, const u16 *tq,
+                                                const u16 *tg, int row0)
+{
+    constexpr int N = DP / 16;  // (16 rows, 32 channels) steps
+    bf8 g[2], q[2];
+    g[0] = ln.transposed(tg, row0, 0), q[0] = ln.transposed(tq, row0, 0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int u = n / (DP / 32), i = n % (DP / 32);
+        if (n + 1 < N) {
+            const int u1 = (n + 1) / (DP / 32), i1 = (n + 1) % (DP / 32);
+            g[(n + 1) & 1] = ln.transposed(tg, row0 + 16 * u1, i1), q[(n + 1) & 1] = ln.transposed(tq, row0 + 16 * u1, i1);
+        }
+        xa_keep();
+        dv[i] = PCM_MFMA16(g[n & 1], xa_pack(p, u), dv[i]);
+        dk[i] = PCM_MFMA16(q[n & 1], xa_pack(ds, u), dk[i]);
+        xa_keep();
+    }
+}
 template <int DP>
 __device__ __forceinline__ void xa_store_keys(const XaParams &P, const XaKeys &K, int key, int h, const f16v (&dk)[DP / 32], const f16v (&dv)[DP / 32])
 {
@@ -785,22 +843,10 @@ __global__ void __launch_bounds__(512, 2) pcm_xattn_dkv_wide_kernel(XaParams P)
     const auto body = [&](int buf, const u16 *tq, const u16 *tg) {
         if (!work) return;
         const XaLane<DP> ln = ln0.here();
-        f16v s = xa_zero16(), dp = xa_zero16();
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) {
-            s = PCM_MFMA16(ln.rows(tq, 32 * half, t), ln.rows(sk, 32 * kg, t), s);
-            dp = PCM_MFMA16(ln.rows(tg, 32 * half, t), ln.rows(sv, 32 * kg, t), dp);
-        }
-        xa_weights(s, dp, sl[buf] + 32 * half, sd[buf] + 32 * half, c, seen, h);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const bf8 p = xa_pack(s, u), ds = xa_pack(dp, u);
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                dv[i] = PCM_MFMA16(ln.transposed(tg, 32 * half + 16 * u, i), p, dv[i]);
-                dk[i] = PCM_MFMA16(ln.transposed(tq, 32 * half + 16 * u, i), ds, dk[i]);
-            }
-        }
+        f16v s[2] = {xa_zero16(), xa_zero16()};  // scores, dP
+        xa_products<DP>(s, [&](int n, int t) { return ln.rows(n ? tg : tq, 32 * half, t); }, [&](int n, int t) { return ln.rows(n ? sv : sk, 32 * kg, t); });
+        xa_weights(s[0], s[1], sl[buf] + 32 * half, sd[buf] + 32 * half, c, seen, h);
+        xa_key_products<DP>(dk, dv, s[0], s[1], ln, tq, tg, 32 * half);
     };
     rows.run(sq0, sg0, sq1, sg1, sl, sd, body);
     // the two halves: [register][lane], dK and then dV, 128 * DP values in the place of K and V
@@ -857,22 +903,10 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dkv_narrow_kernel(XaParams P
         const XaLane<DP> ln = ln0.here();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f16v s = xa_zero16(), dp = xa_zero16();
-#pragma unroll
-            for (int t = 0; t < DP / 16; ++t) {
-                s = PCM_MFMA16(ln.rows(tq, 32 * j, t), kf[t], s);
-                dp = PCM_MFMA16(ln.rows(tg, 32 * j, t), vf[t], dp);
-            }
-            xa_weights(s, dp, sl[buf] + 32 * j, sd[buf] + 32 * j, c, seen, h);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const bf8 p = xa_pack(s, u), ds = xa_pack(dp, u);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
-                    dv[i] = PCM_MFMA16(ln.transposed(tg, 32 * j + 16 * u, i), p, dv[i]);
-                    dk[i] = PCM_MFMA16(ln.transposed(tq, 32 * j + 16 * u, i), ds, dk[i]);
-                }
-            }
+            f16v s[2] = {xa_zero16(), xa_zero16()};
+            xa_products<DP>(s, [&](int n, int t) { return ln.rows(n ? tg : tq, 32 * j, t); }, [&](int n, int t) { return n ? vf[t] : kf[t]; });
+            xa_weights(s[0], s[1], sl[buf] + 32 * j, sd[buf] + 32 * j, c, seen, h);
+            xa_key_products<DP>(dk, dv, s[0], s[1], ln, tq, tg, 32 * j);
         }
     };
     rows.run(sq0, sg0, sq1, sg1, sl, sd, body);
