@@ -17,7 +17,7 @@
 // image (S = Q K^T: a lane owns one key).  Nothing is ever transposed through registers or a second LDS copy.
 //
 // Masked or absent keys are zeroed in K and V where a tile is staged (a NaN or infinity in padding must not meet a zero weight) and
-// their scores are replaced by -inf.  Sums, maxima, lse, delta and accumulators are fp32; P and dS are rounded to bf16 (one half step,
+// their scores start from -inf.  Sums, maxima, lse, delta and accumulators are fp32; P and dS are rounded to bf16 (one half step,
 // 2^-8 relative at most) because the matrix operands are bf16; outputs are rounded once; delta reads O as it was stored (its rounding's
 // part of dQ is a fraction of dS's own: O is an average of V).
 #include "pcm_attn.hpp"
@@ -121,17 +121,19 @@ __device__ __forceinline__ void xa_row_operand(const u16 *row, bool ok, int D, i
         f[t] = as_bf8(ok && 16 * t + 8 * h < D ? *(const uint4 *)(row + 16 * t + 8 * h) : make_uint4(0, 0, 0, 0));
 }
 
-// Tiles of 64 rows x DP channels in LDS, filled by global_load_lds: a wave's 64 16-byte pieces go to consecutive addresses, no registers
+// Tiles of 64 rows x DP channels in LDS, filled by buffer_load ... lds: a wave's 64 16-byte pieces go to consecutive addresses, no registers
 // and no LDS write instructions.  That layout cannot be padded, so the piece a slot holds is permuted by its row (the lane picks its
-// source), see xa_swz.  Pieces outside (absent or masked rows, channels from D on) are read from a block of zeros.
-__device__ uint4 xa_zeros;
+// source), see xa_swz.  The descriptor starts at the tile's first row and covers 2 GB; a lane has one 32-bit offset a piece.  Pieces outside
+// (absent or masked rows, channels from D on) get an offset behind it, which reads zeros: one selection where 64-bit addresses took six
+// operations, with holes in the mask a sixth of the row kernels' vector instructions.
 typedef __attribute__((address_space(3))) void *xa_lds_p;
-typedef const __attribute__((address_space(1))) void *xa_glb_p;
-typedef const __attribute__((address_space(1))) char *xa_glb_c;
-__device__ __forceinline__ const u16 *xa_uniform(const u16 *p)  // the same in all lanes: to scalar registers
+constexpr unsigned XA_SPAN = 0x7FFFFFFFu, XA_OUT = 0x80000000u;
+constexpr long XA_NEAR = 1 << 22;  // strides below it: 128 rows, 64 tokens and their heads are less than 2 GB apart
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t xa_from(const u16 *p)  // p: the same in all lanes
 {
     const uint64_t a = (uint64_t)p;
-    return (const u16 *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)a));
+    const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)u, 0, XA_SPAN, 0x00027000);  // raw, 32-bit data
 }
 
 // 64 banks of 4 bytes.  ds_read_b128 serves the lanes 0-3, 12-15, 20-23, 24-27 of 32 together, then the other 16: the rows of either set
@@ -149,8 +151,6 @@ __device__ __forceinline__ int xa_at(int row, int piece)  // value offset of a p
     return row * DP + ((piece ^ xa_swz<DP>(row)) << 3);
 }
 
-constexpr long XA_NEAR = 1 << 23;  // 64 rows at smaller strides are less than 2^31 bytes apart
-
 // THREADS threads (a workgroup or one wave) request ROWS rows; a thread's n-th piece stands n * NR rows below its first.
 template <int DP, int ROWS, int THREADS>
 struct XaStage {
@@ -158,58 +158,43 @@ struct XaStage {
     int r;        // tile row of the first piece
     int p;        // its channel
     int dim;
-    static_assert((NR & (NR - 1)) == 0 && ROWS % NR == 0, "see load()");
+    static_assert((NR & (NR - 1)) == 0 && ROWS % NR == 0, "r < NR and NR is a power of two: the permutation's bits separate");
     __device__ __forceinline__ void init(int t, int D)
     {
         r = t / PIECES, p = 8 * ((t - r * PIECES) ^ xa_swz<DP>(r)), dim = D;
     }
-    static __device__ __forceinline__ void put(const u16 *src, bool ok, u16 *tile, int n, int wave)
+    __device__ __forceinline__ int channel(int n) const { return p ^ (8 * xa_swz<DP>(n * NR)); }
+    static __device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t from, unsigned at, u16 *tile, int n, int wave)
     {
-        __builtin_amdgcn_global_load_lds((xa_glb_p)(ok ? (const void *)src : (const void *)&xa_zeros), (xa_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, 0, 0);
-    }
-    // All rows from `src` on at stride ls < XA_NEAR are wanted, all DP channels: one 32-bit offset a lane beside uniform addresses, and no
-    // selection.  With the general form below, addresses were a fifth of the row kernels' vector instructions.
-    __device__ __forceinline__ void load_all(const u16 *src, int ls, u16 *tile, int wave) const
-    {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const unsigned at = 2u * (unsigned)(r * ls + (p ^ (8 * xa_swz<DP>(n * NR))));
-            const xa_glb_c row = (xa_glb_c)(const char *)xa_uniform(src + (long)(n * NR) * ls);
-            __builtin_amdgcn_global_load_lds((xa_glb_p)(row + at), (xa_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, 0, 0);
-        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (xa_lds_p)(tile + (n * THREADS + wave * 64) * 8), 16, at, 0, 0, 0);
     }
     // rows row0 .. of a matrix at row stride ls; visible: bit i <-> tile row i
     __device__ __forceinline__ void load(const u16 *base, long ls, long row0, unsigned long long visible, u16 *tile, int wave) const
     {
-        if (visible == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1) && dim == DP && ls < XA_NEAR) return load_all(base + row0 * ls, (int)ls, tile, wave);
-        const u16 *src = base + (row0 + r) * ls;
+        const __amdgpu_buffer_rsrc_t from = xa_from(base + row0 * ls);
+        const bool all = visible == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1);
         const unsigned long long mine = visible >> r;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int pn = p ^ (8 * xa_swz<DP>(n * NR));  // r < NR and NR is a power of two: the permutation's bits separate
-            put(src + n * (NR * ls) + pn, pn < dim && ((mine >> (n * NR)) & 1), tile, n, wave);
+            const int c = channel(n);
+            unsigned at = 2u * (unsigned)((r + n * NR) * (int)ls + c);
+            if (c >= dim) at = XA_OUT;
+            if (!all) at = (mine >> (n * NR)) & 1 ? at : XA_OUT;
+            put(from, at, tile, n, wave);
         }
     }
-};
-// rows = token * G + g of a (token, head, channel) matrix
-template <int DP, int ROWS, int THREADS>
-struct XaRowStage : XaStage<DP, ROWS, THREADS> {
-    typedef XaStage<DP, ROWS, THREADS> Base;
-    __device__ __forceinline__ void load_rows(const u16 *a, long a_ls, long a_hs, u16 *ta, const u16 *b, long b_ls, long b_hs, u16 *tb, int row0, int n, const XaParams &P, int wave) const
+    // rows = token * G + g of two (token, head, channel) matrices
+    __device__ __forceinline__ void load_rows(const u16 *a, long a_ls, long a_hs, u16 *ta, const u16 *b, long b_ls, long b_hs, u16 *tb, int row0, int n,
+                                              const XaParams &P, int wave) const
     {
-        // one head a key head, or all of them: rows at one stride
-        const long as = P.G == 1 ? a_ls : a_hs, bs = P.G == 1 ? b_ls : b_hs;
-        if (row0 + ROWS <= n && Base::dim == DP && (P.G == 1 || (a_ls == P.G * a_hs && b_ls == P.G * b_hs)) && as < XA_NEAR && bs < XA_NEAR) {
-            Base::load_all(a + row0 * as, (int)as, ta, wave), Base::load_all(b + row0 * bs, (int)bs, tb, wave);
-            return;
-        }
+        const int tok0 = P.token(row0);
+        const __amdgpu_buffer_rsrc_t af = xa_from(a + tok0 * a_ls), bf = xa_from(b + tok0 * b_ls);
 #pragma unroll
-        for (int i = 0; i < Base::N; ++i) {
-            const int row = row0 + Base::r + i * Base::NR, tok = P.token(row), g = row - tok * P.G;
-            const int pn = Base::p ^ (8 * xa_swz<DP>(i * Base::NR));
-            const bool ok = pn < Base::dim && row < n;
-            Base::put(a + tok * a_ls + g * a_hs + pn, ok, ta, i, wave);
-            Base::put(b + tok * b_ls + g * b_hs + pn, ok, tb, i, wave);
+        for (int i = 0; i < N; ++i) {
+            const int row = row0 + r + i * NR, tok = P.token(row), g = row - tok * P.G, c = channel(i);
+            const bool ok = c < dim && row < n;
+            put(af, ok ? 2u * (unsigned)((tok - tok0) * (int)a_ls + g * (int)a_hs + c) : XA_OUT, ta, i, wave);
+            put(bf, ok ? 2u * (unsigned)((tok - tok0) * (int)b_ls + g * (int)b_hs + c) : XA_OUT, tb, i, wave);
         }
     }
 };
@@ -226,13 +211,18 @@ __device__ __forceinline__ unsigned long long xa_visible(const unsigned char *ma
     const int left = n - key0;
     return left >= 64 ? ~0ull : (left <= 0 ? 0ull : (1ull << left) - 1);
 }
-// scores of keys that are not to be seen
-__device__ __forceinline__ void xa_hide(f16v &s, unsigned keys, int h, float v)
+// What the scores of 32 keys start from: 0, or -inf for keys that are not to be seen (their K and V are zeros).  A matrix instruction adds to it,
+// so a hole in the mask costs four LDS reads of the keys' biases instead of a test and a selection a score.
+__device__ __forceinline__ float xa_bias(unsigned long long visible, int i) { return (visible >> i) & 1 ? 0.f : -INFINITY; }
+__device__ __forceinline__ f16v xa_start(const float *bias, int h)
 {
-    const unsigned mine = keys >> (4 * h);
+    f16v s;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-        if (!((mine >> ((r & 3) + 8 * (r >> 2))) & 1)) s[r] = v;
+    for (int g = 0; g < 4; ++g) {
+        const float4 b = *(const float4 *)(bias + 8 * g + 4 * h);
+        s[4 * g] = b.x, s[4 * g + 1] = b.y, s[4 * g + 2] = b.z, s[4 * g + 3] = b.w;
+    }
+    return s;
 }
 
 // Transposed operand: lane <-> channel 32 * blk + lane % 32, contracted index i of half h <-> tile row row16 + 4 h + i % 4 + 8 (i / 4):
@@ -363,21 +353,25 @@ struct XaSoftmax {
     }
     // NJ * 32 keys of a tile, c = scale * log2 e
     template <int NJ>
-    __device__ __forceinline__ void tile(const u16 *sk, const u16 *sv, const bf8 (&qf)[DP / 16], unsigned long long vis, float c, const XaLane<DP> &ln0, int h)
+    __device__ __forceinline__ void tile(const u16 *sk, const u16 *sv, const bf8 (&qf)[DP / 16], bool all, const float *bias, float c, const XaLane<DP> &ln0, int h)
     {
         const XaLane<DP> ln = ln0.here();
         f16v s[NJ];
+        const auto keys = [&](int j, int t) { return ln.rows(sk, 32 * j, t); };
+        const auto rows = [&](int, int t) { return qf[t]; };
+        if (all) {  // twice, so that zeros need no registers: a matrix instruction takes the constant
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) s[j] = xa_zero16();
-        xa_products<DP>(s, [&](int j, int t) { return ln.rows(sk, 32 * j, t); }, [&](int, int t) { return qf[t]; });
+            for (int j = 0; j < NJ; ++j) s[j] = xa_zero16();
+            xa_products<DP>(s, keys, rows);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) s[j] = xa_start(bias + 32 * j, h);
+            xa_products<DP>(s, keys, rows);
+        }
         bf8 vt[2][DP / 32];
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) vt[0][i] = ln.transposed(sv, 0, i);
         xa_keep();
-        if (vis != (NJ == 2 ? ~0ull : 0xFFFFFFFFull)) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) xa_hide(s[j], (unsigned)(vis >> (32 * j)), h, -INFINITY);
-        }
         float mx = m;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
@@ -437,37 +431,40 @@ __device__ __forceinline__ void xa_finish(const XaParams &P, const XaRows &R, co
 // The keys of a row kernel, 64 at a time through two LDS buffers of K and V: while tile t is worked on, tile t + 1 is on its way.  The
 // buffers are variables of their own, so that the compiler can tell reads of one from requests into the other.
 template <int DP, class F>
-__device__ __forceinline__ void xa_key_loop(const XaRows &R, const XaParams &P, u16 *sk0, u16 *sv0, u16 *sk1, u16 *sv1, int lane, int wave, F body)
+__device__ __forceinline__ void xa_key_loop(const XaRows &R, const XaParams &P, u16 *sk0, u16 *sv0, u16 *sk1, u16 *sv1, float (*bias)[XA_TILE], int lane, int wave,
+                                            F body)
 {
     if (R.key_lo >= R.key_hi) return;
     XaStage<DP, XA_TILE, 256> st;
     st.init((int)threadIdx.x, P.D);
     unsigned mb = xa_mask_byte(R.mask, R.key_lo + lane, R.ks.n);
     unsigned long long next = 0;
-    const auto request = [&](int key0, u16 *tk, u16 *tv) {
+    const auto request = [&](int key0, u16 *tk, u16 *tv, float *tb) {
         next = xa_visible(R.mask, mb, key0, R.ks.n, lane);
+        if (next != ~0ull && wave == 0) tb[lane] = xa_bias(next, lane);
         st.load(R.k, P.k_ls, key0, next, tk, wave), st.load(R.v, P.v_ls, key0, next, tv, wave);
         mb = xa_mask_byte(R.mask, key0 + XA_TILE + lane, R.ks.n);
     };
-    const auto step = [&](int key0, const u16 *tk, const u16 *tv, u16 *nk, u16 *nv) {
+    const auto step = [&](int key0, int buf, const u16 *tk, const u16 *tv, u16 *nk, u16 *nv) {
         xa_arrived();
         const unsigned long long vis = next;
-        if (key0 + XA_TILE < R.key_hi) request(key0 + XA_TILE, nk, nv);
-        if (vis != 0 && R.work) body(tk, tv, vis);
+        if (key0 + XA_TILE < R.key_hi) request(key0 + XA_TILE, nk, nv, bias[1 - buf]);
+        if (vis != 0 && R.work) body(tk, tv, vis == ~0ull, bias[buf]);
     };
-    request(R.key_lo, sk0, sv0);
+    request(R.key_lo, sk0, sv0, bias[0]);
     int key0 = R.key_lo;
     for (; key0 + XA_TILE < R.key_hi; key0 += 2 * XA_TILE) {
-        step(key0, sk0, sv0, sk1, sv1);
-        step(key0 + XA_TILE, sk1, sv1, sk0, sv0);
+        step(key0, 0, sk0, sv0, sk1, sv1);
+        step(key0 + XA_TILE, 1, sk1, sv1, sk0, sv0);
     }
-    if (key0 < R.key_hi) step(key0, sk0, sv0, sk1, sv1);
+    if (key0 < R.key_hi) step(key0, 0, sk0, sv0, sk1, sv1);
 }
 
 template <int DP>
 __global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
 {
     __shared__ __attribute__((aligned(1024))) u16 sk0[XA_TILE * DP], sv0[XA_TILE * DP], sk1[XA_TILE * DP], sv1[XA_TILE * DP];
+    __shared__ __attribute__((aligned(16))) float bias[2][XA_TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
     const XaLane<DP> ln(lane);
     XaRows R;
@@ -477,8 +474,8 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
     XaSoftmax<DP> w;
     w.init();
     const float c = P.scale * XA_LOG2E;
-    xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, lane, wave,
-                    [&](const u16 *tk, const u16 *tv, unsigned long long vis) { w.template tile<2>(tk, tv, qf, vis, c, ln, h); });
+    xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, bias, lane, wave,
+                    [&](const u16 *tk, const u16 *tv, bool all, const float *tb) { w.template tile<2>(tk, tv, qf, all, tb, c, ln, h); });
     w.l += __shfl_xor(w.l, 32);
     xa_finish<DP>(P, R, w.o, w.m, w.l, h);
 }
@@ -492,6 +489,7 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
     constexpr int TILE = 32 * DP;
     __shared__ __attribute__((aligned(1024))) u16 t0[4 * 2 * TILE], t1[4 * 2 * TILE];
     __shared__ float sm[4][32], sl[4][32];
+    __shared__ __attribute__((aligned(16))) float bias[4][2][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     const XaLane<DP> ln(lane);
     XaRows R;
@@ -506,28 +504,29 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
     u16 *const k0 = t0 + wave * 2 * TILE, *const k1 = t1 + wave * 2 * TILE;
     unsigned mb = 0;
     unsigned long long vis = 0, next = 0;
-    const auto request = [&](int key0, u16 *tk) {
+    const auto request = [&](int key0, u16 *tk, float *tb) {
         next = xa_visible(R.mask, mb, key0, R.ks.n, lane) & 0xFFFFFFFFull;
+        if (next != 0xFFFFFFFFull && lane < 32) tb[lane] = xa_bias(next, lane);
         st.load(R.k, P.k_ls, key0, next, tk, 0), st.load(R.v, P.v_ls, key0, next, tk + TILE, 0);
         mb = xa_mask_byte(R.mask, key0 + 128 + lane, R.ks.n);
     };
-    const auto step = [&](int key0, const u16 *tk, u16 *nk) {
+    const auto step = [&](int key0, int buf, const u16 *tk, u16 *nk) {
         __builtin_amdgcn_s_waitcnt(0x70);  // this wave's tile has arrived, its reads of the other are done
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         vis = next;
-        if (key0 + 128 < R.key_hi) request(key0 + 128, nk);
-        if (vis != 0) w.template tile<1>(tk, tk + TILE, qf, vis, c, ln, h);
+        if (key0 + 128 < R.key_hi) request(key0 + 128, nk, bias[wave][1 - buf]);
+        if (vis != 0) w.template tile<1>(tk, tk + TILE, qf, vis == 0xFFFFFFFFull, bias[wave][buf], c, ln, h);
     };
     int key0 = R.key_lo + 32 * wave;
     if (key0 < R.key_hi) {
         mb = xa_mask_byte(R.mask, key0 + lane, R.ks.n);
-        request(key0, k0);
+        request(key0, k0, bias[wave][0]);
         for (; key0 + 128 < R.key_hi; key0 += 256) {
-            step(key0, k0, k1);
-            step(key0 + 128, k1, k0);
+            step(key0, 0, k0, k1);
+            step(key0 + 128, 1, k1, k0);
         }
-        if (key0 < R.key_hi) step(key0, k0, k1);
+        if (key0 < R.key_hi) step(key0, 0, k0, k1);
     }
     w.l += __shfl_xor(w.l, 32);
     if (h == 0) sm[wave][col] = w.m, sl[wave][col] = w.l;
@@ -599,6 +598,7 @@ template <int DP>
 __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
 {
     __shared__ __attribute__((aligned(1024))) u16 sk0[XA_TILE * DP], sv0[XA_TILE * DP], sk1[XA_TILE * DP], sv1[XA_TILE * DP];
+    __shared__ __attribute__((aligned(16))) float bias[2][XA_TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
     const XaLane<DP> ln0(lane);
     XaRows R;
@@ -623,12 +623,19 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
     f16v o[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = xa_zero16();
-    xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, lane, wave, [&](const u16 *tk, const u16 *tv, unsigned long long vis) {
+    xa_key_loop<DP>(R, P, sk0, sv0, sk1, sv1, bias, lane, wave, [&](const u16 *tk, const u16 *tv, bool all, const float *tb) {
         const XaLane<DP> ln = ln0.here();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             f16v s[2] = {xa_zero16(), xa_zero16()};  // scores, dP
-            xa_products<DP>(s, [&](int n, int t) { return ln.rows(n ? tv : tk, 32 * j, t); }, [&](int n, int t) { return n ? gf[t] : qf[t]; });
+            const auto keys = [&](int n, int t) { return ln.rows(n ? tv : tk, 32 * j, t); };
+            const auto rows = [&](int n, int t) { return n ? gf[t] : qf[t]; };
+            if (all) {
+                xa_products<DP>(s, keys, rows);
+            } else {
+                s[0] = xa_start(tb + 32 * j, h);
+                xa_products<DP>(s, keys, rows);
+            }
             bf8 kt[2][DP / 32];
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) kt[0][i] = ln.transposed(tk, 32 * j, i);
@@ -638,7 +645,6 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c, -l2));
                 s[0][r] = p * (s[1][r] - delta);
             }
-            if (vis != ~0ull) xa_hide(s[0], (unsigned)(vis >> (32 * j)), h, 0.f);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if (u == 0) {
@@ -712,7 +718,7 @@ struct XaRowLoop {
     const XaParams &P;
     const XaKeys &K;
     const int wave;
-    XaRowStage<DP, XA_TILE, ROWT> st;
+    XaStage<DP, XA_TILE, ROWT> st;
     const u16 *qb, *gb;
     float rl, rd;
     __device__ __forceinline__ XaRowLoop(const XaParams &P_, const XaKeys &K_, int wave_) : P(P_), K(K_), wave(wave_), qb(nullptr), gb(nullptr)
@@ -830,12 +836,13 @@ __global__ void __launch_bounds__(512, 2) pcm_xattn_dkv_wide_kernel(XaParams P)
     if (K.lo < K.nrows) {  // K and V, zeros for keys that are not there or not seen
         XaStage<DP, XA_ROWS, 512> kt;
         kt.init((int)threadIdx.x, P.D);
-        const u16 *kp = P.k + K.kb * P.k_bs + K.kr * P.k_ls + (long)K.kvh * P.k_hs, *vp = P.v + K.kb * P.v_bs + K.kr * P.v_ls + (long)K.kvh * P.v_hs;
+        const __amdgpu_buffer_rsrc_t kf = xa_from(P.k + K.kb * P.k_bs + (K.kr + K.key0) * P.k_ls + (long)K.kvh * P.k_hs),
+                                     vf = xa_from(P.v + K.kb * P.v_bs + (K.kr + K.key0) * P.v_ls + (long)K.kvh * P.v_hs);
 #pragma unroll
         for (int n = 0; n < kt.N; ++n) {
-            const int j = K.key0 + kt.r + n * kt.NR, pn = kt.p ^ (8 * xa_swz<DP>(n * kt.NR));
-            const bool ok = pn < P.D && j < K.ks.n && (K.mask == nullptr || K.mask[j] == 0);
-            kt.put(kp + (long)j * P.k_ls + pn, ok, sk, n, wave), kt.put(vp + (long)j * P.v_ls + pn, ok, sv, n, wave);
+            const int i = kt.r + n * kt.NR, j = K.key0 + i, c = kt.channel(n);
+            const bool ok = c < P.D && j < K.ks.n && (K.mask == nullptr || K.mask[j] == 0);
+            kt.put(kf, ok ? 2u * (unsigned)(i * (int)P.k_ls + c) : XA_OUT, sk, n, wave), kt.put(vf, ok ? 2u * (unsigned)(i * (int)P.v_ls + c) : XA_OUT, sv, n, wave);
         }
     }
     XaRowLoop<DP, 512> rows(P, K, wave);
@@ -978,7 +985,11 @@ int xa_row_splits(int B, int Hkv, int G, long q_rows, int S, long kv_rows, int k
 }
 int xa_row_splits(const XaParams &P) { return xa_row_splits(P.B, P.Hkv, P.G, P.q_rows, P.S, P.kv_rows, P.kv_off != nullptr); }
 
-bool xa_strides_ok(const void *p, long bs, long ls, long hs) { return (((uintptr_t)p) & 15) == 0 && ((bs | ls | hs) & 7) == 0; }
+// heads: those of a key head where a tile holds several (queries)
+bool xa_strides_ok(const void *p, long bs, long ls, long hs, long heads)
+{
+    return (((uintptr_t)p) & 15) == 0 && ((bs | ls | hs) & 7) == 0 && ls >= 0 && hs >= 0 && ls < XA_NEAR && hs * (heads - 1) < 1L << 29;
+}
 
 int xa_fill(XaParams &P, int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows, const int *kv_offset,
             const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs, long k_ls, long k_hs, const void *v, long v_bs, long v_ls,
@@ -996,7 +1007,7 @@ int xa_fill(XaParams &P, int B, int H, int Hkv, int D, int L, long q_rows, const
         xa_tiles(kv_offset != nullptr, B, S, kv_rows, 1, XA_ROWS) > 0xFFFFF000L / 512 / Hkv)
         return PCM_ERR_UNSUPPORTED;
     if ((q_rows > 0 && !q) || (kv_rows > 0 && (!k || !v))) return PCM_ERR_BAD_ARG;
-    if (!xa_strides_ok(q, q_bs, q_ls, q_hs) || !xa_strides_ok(k, k_bs, k_ls, k_hs) || !xa_strides_ok(v, v_bs, v_ls, v_hs)) return PCM_ERR_UNSUPPORTED;
+    if (!xa_strides_ok(q, q_bs, q_ls, q_hs, H / Hkv) || !xa_strides_ok(k, k_bs, k_ls, k_hs, 1) || !xa_strides_ok(v, v_bs, v_ls, v_hs, 1)) return PCM_ERR_UNSUPPORTED;
     P.q = (const u16 *)q, P.k = (const u16 *)k, P.v = (const u16 *)v;
     P.q_bs = q_bs, P.q_ls = q_ls, P.q_hs = q_hs, P.k_bs = k_bs, P.k_ls = k_ls, P.k_hs = k_hs, P.v_bs = v_bs, P.v_ls = v_ls, P.v_hs = v_hs;
     P.mask = mask, P.mask_bs = mask_bs, P.q_off = q_offset, P.kv_off = kv_offset;
@@ -1069,7 +1080,7 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
     if (bad) return bad;
     if (P.q_rows > 0 && (!out || !lse || !dout || !delta || !dq)) return PCM_ERR_BAD_ARG;
     if (P.kv_rows > 0 && (!dk || !dv)) return PCM_ERR_BAD_ARG;
-    if (!xa_strides_ok(dout, g_bs, g_ls, g_hs)) return PCM_ERR_UNSUPPORTED;
+    if (!xa_strides_ok(dout, g_bs, g_ls, g_hs, H / Hkv)) return PCM_ERR_UNSUPPORTED;
     if ((((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
     P.out = (u16 *)out, P.lse = (float *)lse, P.dout = (const u16 *)dout, P.g_bs = g_bs, P.g_ls = g_ls, P.g_hs = g_hs;
     P.delta = delta, P.dq = (u16 *)dq, P.dk = (u16 *)dk, P.dv = (u16 *)dv;

@@ -15,16 +15,20 @@ from .._lib import raw_stream as _raw_stream
 MAX_HEAD_DIM = 128
 
 
-def _fit(t):
-    """(t, (batch, row, head) strides in elements, 0 where there is one entry only); t a contiguous copy where the kernels' 16-byte
-    accesses do not fit its strides or address."""
+def _fit(t, group=1):
+    """(t, (batch, row, head) strides in elements, 0 where there is one entry only); t a contiguous copy where its strides or address do
+    not fit the kernels' 16-byte accesses, or rows (and the `group` heads of a key head) lie too far apart for offsets of 32 bits in a tile."""
     *st, last = t.stride()
-    if last != 1 or t.data_ptr() % 16 or any(s % 8 for s in st):
+    if not _fits(t, st, last, group):
         st = [s if n > 1 else 0 for s, n in zip(st, t.shape)]
-        if last != 1 or t.data_ptr() % 16 or any(s % 8 for s in st):
+        if not _fits(t, st, last, group):
             t = t.clone(memory_format=torch.contiguous_format)
             st = t.stride()[:-1]
     return t, (st if len(st) == 3 else (0, *st))
+
+
+def _fits(t, st, last, group):
+    return last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in st) and st[-2] < 1 << 22 and st[-1] * (group - 1) < 1 << 29
 
 
 def _new(t):
@@ -33,8 +37,8 @@ def _new(t):
 
 def _arguments(q, k, v, mask, q_offset, kv_offset, scale):
     """The operands as the kernels take them, the arguments that describe them, and the bytes of workspace of either direction."""
-    (q, qs), (k, ks), (v, vs) = _fit(q), _fit(k), _fit(v)
     qshape, kshape = q.shape, k.shape
+    (q, qs), (k, ks), (v, vs) = _fit(q, qshape[-2] // kshape[-2]), _fit(k), _fit(v)
     h, d, hkv = qshape[-2], qshape[-1], kshape[-2]
     b, l, q_rows, qo = (qshape[0], qshape[1], qshape[0] * qshape[1], 0) if len(qshape) == 4 else (q_offset.numel(), 0, qshape[0], q_offset.data_ptr())
     s, kv_rows, ko = (kshape[1], kshape[0] * kshape[1], 0) if len(kshape) == 4 else (0, kshape[0], kv_offset.data_ptr())
@@ -73,7 +77,7 @@ class _CrossAttention(Function):
         dev = q.device
         with _lib.on_device(dev):
             q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale)
-            dout, gs = _fit(dout)
+            dout, gs = _fit(dout, q.shape[-2] // k.shape[-2])
             dq, dk, dv = _new(q), _new(k), _new(v)
             at = lse.numel() * 4 + 15 & ~15
             ws = torch.empty(at + ws_bytes, dtype=torch.uint8, device=dev)  # delta, then the workspace

@@ -232,3 +232,24 @@ def test_long_states_under_many_rows_at_size():
     mask = torch.zeros(8300, dtype=torch.bool)
     mask[100:2400] = True
     _check(*_inputs((4700,), (8300,), 4, 16, 8, seed=24), mask, [2300, 2400], [4200, 4100])
+
+
+def test_rows_far_apart():
+    """Row strides of 2^22 values and more are copied first; just below them, rows of a tile are up to 2^30 bytes apart."""
+    q, k, v, dout = _inputs((1, 3), (1, 5), 1, 32, 2, seed=25)
+    want = _run(q, k, v, dout, None, None, None)
+    for step in ((1 << 22) - 8, 1 << 22):
+        def far(t):
+            rows = torch.zeros((t.shape[1] - 1) * step + t[0, 0].numel(), dtype=t.dtype, device=DEV)
+            view = rows.as_strided(t.shape, (0, step, t.shape[3], 1))
+            return view.copy_(t.to(DEV))
+
+        got = _run(*(far(t) for t in (q, k, v, dout)), None, None, None)
+        assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[2], want[2])), step
+
+
+def test_rows_shared_by_all_positions():
+    """A stride of zero: one key and value for every position, which average to that value."""
+    q, k, v, dout = _inputs((2, 9), (2, 1), 2, 64, 4, seed=26)
+    wide = lambda t: t.expand(2, 70, 2, 64)  # noqa: E731
+    _check(q, wide(k), wide(v), dout, None, None, None, leaves=(q, wide(k.to(DEV)), wide(v.to(DEV)), dout))

@@ -161,6 +161,21 @@ template <class P> inline __attribute__((always_inline)) ws_s4 ws_ds_read_tr16(P
 #define __builtin_amdgcn_global_load_lds(g, l, size, off, aux) \
     std::memcpy((char *)(void *)(l) + (off) + (size) * wavesim::g_cur->lane, (const char *)(const void *)(g) + (off), (size))
 
+// buffer_load ... lds: the same through a descriptor; offsets outside its bytes read zeros (raw buffers, each offset a multiple of 16)
+struct ws_rsrc {
+    const char *base;
+    uint32_t bytes;
+};
+#define __amdgpu_buffer_rsrc_t ws_rsrc
+#define __builtin_amdgcn_make_buffer_rsrc(p, stride, num, flags) (ws_rsrc{(const char *)(p), (uint32_t)(num)})
+inline void ws_buffer_load_lds(ws_rsrc r, void *l, uint32_t size, uint32_t at)
+{
+    char *to = (char *)l + size * (uint32_t)wavesim::g_cur->lane;
+    if (at < r.bytes) std::memcpy(to, r.base + at, size);
+    else std::memset(to, 0, size);
+}
+#define __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, size, voff, soff, imm, aux) ws_buffer_load_lds((r), (void *)(l), (size), (voff) + (soff) + (imm))
+
 // matrix instructions: every lane deposits its operand registers, the resolver multiplies with the ISA's operand layouts (wavesim.cpp)
 typedef float ws_f16v __attribute__((ext_vector_type(16)));
 typedef float ws_f4v __attribute__((ext_vector_type(4)));
