@@ -104,6 +104,9 @@ def captured(fn, pool=None):
     return graph, result
 
 
+_ACCUMULATE = torch._C._functions.AccumulateGrad
+
+
 def guard_leaves(out, what):
     """`out`, the result of an autograd function whose inputs may be leaves, views of them or casts -- refused during a capture when an
     eager graph over the same leaves is alive.  autograd keeps ONE accumulation node per leaf, for as long as any graph holds it, on the
@@ -115,14 +118,16 @@ def guard_leaves(out, what):
     here, capturing = _lib.raw_stream(), torch.cuda.is_current_stream_capturing()
     for node, _ in out.grad_fn.next_functions:
         for _ in range(4):  # through what a wrapper puts in front: a view, a cast, a copy
-            if node is None or len(node.next_functions) != 1:
+            if type(node) is _ACCUMULATE:
+                made = node.metadata.setdefault("pcm_stream", here)
+                if capturing and made != here:
+                    raise RuntimeError("%s: an eager graph over the same leaf tensors is alive: free its outputs before a backward pass "
+                                       "of them is captured" % what)
                 break
-            node = node.next_functions[0][0]
-        if node is not None and not node.next_functions and node.name().endswith("AccumulateGrad"):
-            made = node.metadata.setdefault("pcm_stream", here)
-            if capturing and made != here:
-                raise RuntimeError("%s: an eager graph over the same leaf tensors is alive: free its outputs before a backward pass "
-                                   "of them is captured" % what)
+            behind = node.next_functions if node is not None else ()
+            if len(behind) != 1:
+                break
+            node = behind[0][0]
     return out
 
 

@@ -71,22 +71,28 @@ class _CrossAttention(Function):
         return out, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, mask, q_offset, kv_offset, out, lse = ctx.saved_tensors
-        dev = q.device
-        with _lib.on_device(dev):
-            q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale)
-            dout, gs = _fit(dout, q.shape[-2] // k.shape[-2])
-            dq, dk, dv = _new(q), _new(k), _new(v)
-            at = lse.numel() * 4 + 15 & ~15
-            ws = torch.empty(at + ws_bytes, dtype=torch.uint8, device=dev)  # delta, then the workspace
-            p = ws.data_ptr()
-            rc = _lib.load().pcm_cross_attn_backward_hip(*args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), *gs, p, dq.data_ptr(),
-                                                         dk.data_ptr(), dv.data_ptr(), p + at, ws_bytes, _raw_stream())
-        if rc:
-            _lib.check(rc, "pcm_cross_attn_backward_hip")
-        return dq, dk, dv, None, None, None, None
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout)
+
+
+def _backward(ctx, dout):
+    q, k, v, mask, q_offset, kv_offset, out, lse = ctx.saved_tensors
+    dev = q.device
+    with _lib.on_device(dev):
+        q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale)
+        dout, gs = _fit(dout, q.shape[-2] // k.shape[-2])
+        dq, dk, dv = _new(q), _new(k), _new(v)
+        at = lse.numel() * 4 + 15 & ~15
+        ws = torch.empty(at + ws_bytes, dtype=torch.uint8, device=dev)  # delta, then the workspace
+        p = ws.data_ptr()
+        rc = _lib.load().pcm_cross_attn_backward_hip(*args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), *gs, p, dq.data_ptr(),
+                                                     dk.data_ptr(), dv.data_ptr(), p + at, ws_bytes, _raw_stream())
+    if rc:
+        _lib.check(rc, "pcm_cross_attn_backward_hip")
+    return dq, dk, dv, None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)  # under create_graph: a second derivative is refused; otherwise its checks cost 4 us for nothing
 
 
 def _check_offset(offset, side, t, name):

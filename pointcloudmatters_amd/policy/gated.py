@@ -58,29 +58,36 @@ class _GatedFFN(Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        L_ = _lib.load()
-        x, w_gate, w_up, w_down, hidden = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        (rows, e), f, dev, dtype = x.shape, w_gate.shape[0], x.device, x.dtype
-        dy = _rows(dy, e)
-        with _lib.on_device(dev):
-            new = torch.zeros if rows == 0 else torch.empty  # no rows: no launch, the gradients of the weights are zero
-            dx = new((rows, e), dtype=dtype, device=dev) if need[0] else None
-            dwg, dwu = new((2, f, e), dtype=dtype, device=dev).unbind() if need[1] or need[2] else (None, None)
-            dwd = new((e, f), dtype=dtype, device=dev) if need[3] else None
-            dbg, dbu = new((2, f), dtype=dtype, device=dev).unbind() if need[4] or need[5] else (None, None)
-            dbd = new((e,), dtype=dtype, device=dev) if need[6] else None
-            n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, True)
-            ws = _empty(n, dev)
-            p, size = hidden.data_ptr(), hidden.numel() // 5
-            rc = L_.pcm_gated_ffn_backward_hip(rows, e, f, ctx.act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
-                                               w_down.data_ptr(), p, p + 2 * size, p + 4 * size, dy.data_ptr(), dy.stride(0), _ptr(dx), _ptr(dwg),
-                                               _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), ws.data_ptr(), n, _raw_stream())
-        if rc:
-            _lib.check(rc, "pcm_gated_ffn_backward_hip")
-        return dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dbg if need[4] else None, dbu if need[5] else None, dbd, None
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dy)
+
+
+def _backward(ctx, dy):
+    L_ = _lib.load()
+    x, w_gate, w_up, w_down, hidden = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    (rows, e), f, dev = x.shape, w_gate.shape[0], x.device
+    dy = _rows(dy, e)
+    with _lib.on_device(dev):
+        like = torch.zeros_like if rows == 0 else torch.empty_like  # no rows: no launch, the gradients of the weights are zero
+        bias = w_gate.new_zeros if rows == 0 else w_gate.new_empty
+        dx = x.new_empty((rows, e)) if need[0] else None
+        dwg, dwu = (like(w_gate), like(w_up)) if need[1] or need[2] else (None, None)
+        dwd = like(w_down) if need[3] else None
+        dbg, dbu = (bias(f), bias(f)) if need[4] or need[5] else (None, None)
+        dbd = bias(e) if need[6] else None
+        n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, True)
+        ws = _empty(n, dev)
+        p, size = hidden.data_ptr(), hidden.numel() // 5
+        rc = L_.pcm_gated_ffn_backward_hip(rows, e, f, ctx.act, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
+                                           w_down.data_ptr(), p, p + 2 * size, p + 4 * size, dy.data_ptr(), dy.stride(0), _ptr(dx), _ptr(dwg),
+                                           _ptr(dwu), _ptr(dwd), _ptr(dbg), _ptr(dbu), _ptr(dbd), ws.data_ptr(), n, _raw_stream())
+    if rc:
+        _lib.check(rc, "pcm_gated_ffn_backward_hip")
+    return dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dbg if need[4] else None, dbu if need[5] else None, dbd, None
+
+
+_backward_once = once_differentiable(_backward)  # under create_graph: a second derivative is refused; otherwise its checks cost 4 us for nothing
 
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation="silu"):

@@ -73,6 +73,19 @@ def test_together_against_64_bits():
         assert off <= 16 * ref.HALF, (name, off)
 
 
+def test_second_derivatives_of_attention_and_block_are_refused():
+    from pointcloudmatters_amd.policy import cross_attention, gated_ffn
+
+    n = lambda *s: torch.randn(*s).bfloat16().to(DEV).requires_grad_()  # noqa: E731
+    q, k, x, w, wd = n(1, 3, 2, 32), n(1, 9, 2, 32), n(4, 16), n(24, 16), n(16, 24)
+    for leaf, f in ((q, lambda: cross_attention(q, k, k)), (x, lambda: gated_ffn(x, w, w, wd))):
+        plain = torch.autograd.grad(f().float().pow(2).sum(), leaf)[0]
+        (g,) = torch.autograd.grad(f().float().pow(2).sum(), leaf, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.float().sum().backward()
+
+
 def test_forward_and_backward_captured():
     from pointcloudmatters_amd import _graphs
 
