@@ -650,6 +650,20 @@ GfShape gf_shape(long M, long N, long K, int nsplit, bool wgrad)
     return middle >= 256 ? GF_MIDDLE : GF_SMALL;
 }
 
+// Rows of a product's first launch.  Tiles a little over whole rounds of workgroups (one / two / three a compute unit) leave the last round nearly
+// empty: 16408 rows are 64 row tiles of 256 and 24 rows, 4 rounds and 16 tiles of a fifth.  Where the last round has under a third of a round's
+// tiles and a round is worth the launch (2^24 products a compute unit, some 20 us), its rows are multiplied by a second launch, in smaller tiles
+// and shared-out contractions of its own choice (16408 rows of 512 -> 2048, forward and backward: @@).
+long gf_first_rows(long M, long N, long K)
+{
+    const GfShape t = gf_shape(M, N, K, 1, false);
+    const long per = t.bm == 256 ? 1 : (t.bm == 128 ? 2 : 3), slots = 256 * per, nt = (N + t.bn - 1) / t.bn;
+    const long whole = gf_tiles(M, N, t) / slots, rest = gf_tiles(M, N, t) - whole * slots;
+    if (whole == 0 || rest == 0 || rest * 3 > slots || t.bm * t.bn * per * K < 1L << 24) return M;
+    const long rows = whole * slots / nt * t.bm;
+    return rows < M ? rows : M;
+}
+
 template <int EP, bool ACOL, bool BCOL>
 void gf_launch(const GfParams &P, hipStream_t s)
 {
@@ -660,6 +674,8 @@ void gf_launch(const GfParams &P, hipStream_t s)
     } else if (t.bm == 128) hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 2, 2, 2>), grid, dim3(256), 0, s, P);
     else hipLaunchKernelGGL((pcm_gated_gemm_kernel<EP, ACOL, BCOL, 1, 2, 2>), grid, dim3(256), 0, s, P);
 }
+
+long gf_tile_rows(long M, long N, long K) { const int bm = gf_shape(M, N, K, 1, false).bm; return (M + bm - 1) / bm; }
 
 // adds a product's joining to what closes the pass
 void gf_join(GfClose &c, const GfParams &P)
@@ -687,17 +703,49 @@ int gf_splits(long M, long N, long K)
     n = n < K / 256 ? n : K / 256;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
+// the row products' second launch
+template <int EP, bool BCOL>
+bool gf_launch_rows(GfParams &P, hipStream_t s)  // false: one launch; true: P is the second one
+{
+    const long M = P.M, first = P.nsplit > 1 ? M : gf_first_rows(M, P.N, P.K);
+    P.M = first;
+    if (EP == EP_OUT) P.F = P.osplit = first;
+    gf_launch<EP, false, BCOL>(P, s);
+    if (first == M) return false;
+    P.M = M - first, P.a.p0 += first * P.a.ld, P.a.rows0 -= (int)first;
+    if (EP == EP_OUT) {
+        P.F = P.osplit = P.M, P.out += first * P.ldo, P.nsplit = gf_splits(P.M, P.N, P.K);
+    } else {
+        P.ka = P.ka ? P.ka + first * P.Fp : nullptr, P.ku = P.ku ? P.ku + first * P.Fp : nullptr;
+        if (EP == EP_GLU) P.h += first * P.Fp;
+        if (EP == EP_DGLU) P.out += first * 2 * P.Fp, P.part = P.part ? P.part + gf_tile_rows(first, P.N, P.K) * 4 * P.Fp : nullptr;
+    }
+    gf_launch<EP, false, BCOL>(P, s);
+    return true;
+}
 long gf_part_bytes(long M, long N, long K) { const int n = gf_splits(M, N, K); return n > 1 ? gf_up(n * M * N * 4, 256) : 0; }
+
+// partial sums of a row product: of all of it, or of its second launch
+long gf_row_part_bytes(long M, long N, long K)
+{
+    if (gf_splits(M, N, K) > 1) return gf_part_bytes(M, N, K);
+    const long first = gf_first_rows(M, N, K);
+    return first < M ? gf_part_bytes(M - first, N, K) : 0;
+}
 
 // partial sums of the three backward products, joined together at the end
 long gf_back_part_bytes(long R, int E, int F)
 {
     const long Fp = gf_up(F, 64);
-    return gf_part_bytes(R, E, 2 * Fp) + gf_part_bytes(2 * Fp, E, R) + gf_part_bytes(E, F, R);
+    return gf_row_part_bytes(R, E, 2 * Fp) + gf_part_bytes(2 * Fp, E, R) + gf_part_bytes(E, F, R);
 }
 int gf_slots(long R) { return (int)(R < 64 ? 1 : (R / 32 > 512 ? 512 : R / 32)); }
 // partial rows of da | du: two wave rows per tile row
-long gf_wave_rows(long R, int E, long Fp) { const int bm = gf_shape(R, Fp, gf_up(E, 8), 1, false).bm; return (R + bm - 1) / bm * 2; }
+long gf_wave_rows(long R, int E, long Fp)
+{
+    const long Ep = gf_up(E, 8), first = gf_first_rows(R, Fp, Ep);
+    return 2 * (gf_tile_rows(first, Fp, Ep) + (first < R ? gf_tile_rows(R - first, Fp, Ep) : 0));
+}
 long gf_sum_bytes(long R, int E, long Fp) { return gf_up((gf_wave_rows(R, E, Fp) * 2 * Fp + gf_slots(R) * gf_up(E, 8)) * 4, 256); }
 // 32-bit rows and columns inside a tile; no launch has 2^32 threads (a copy of x, dy and three weights takes one for eight values)
 bool gf_sizes_ok(long R, int E, int F)
@@ -717,7 +765,7 @@ extern "C" long pcm_gated_ffn_ws_bytes(long R, int E, int F, int backward)
     if (!backward && R <= GF_FEW) return 0;
     // copies: x and dy (any strides), the three weights
     long n = gf_pack_bytes(R, E) * (backward ? 2 : 1) + 2 * gf_pack_bytes(F, E) + gf_pack_bytes(E, F);
-    if (!backward) n += gf_part_bytes(R, E, gf_up(F, 8));
+    if (!backward) n += gf_row_part_bytes(R, E, gf_up(F, 8));
     if (backward) {
         n += gf_up(R * 2 * Fp * 2, 256);  // da | du
         n += gf_back_part_bytes(R, E, F);
@@ -751,7 +799,7 @@ extern "C" int pcm_gated_ffn_forward_hip(long R, int E, int F, int act, const vo
     }
     if (ws_bytes < pcm_gated_ffn_ws_bytes(R, E, F, 0) || !ws) return PCM_ERR_BAD_ARG;
     float *const part = (float *)ws;
-    const long part_bytes = gf_part_bytes(R, E, gf_up(F, 8));
+    const long part_bytes = gf_row_part_bytes(R, E, gf_up(F, 8));
     GfPacker pk((char *)ws + part_bytes, ws_bytes - part_bytes);
     long ldx = x_ls, ldg = E, ldu = E, ldd = F;
     const u16 *px = pk.get(x, R, E, ldx);
@@ -764,11 +812,11 @@ extern "C" int pcm_gated_ffn_forward_hip(long R, int E, int F, int act, const vo
     P.a = gf_mat(px, ldx, R, Ep), P.b = gf_mat2(pg, pu, ldg, Fp, F, Ep);
     P.M = R, P.N = 2 * Fp, P.K = Ep, P.act = act, P.nsplit = 1, P.F = F, P.Fp = Fp;
     P.bias0 = (const u16 *)bg, P.bias1 = (const u16 *)bu, P.ka = (float *)a, P.ku = (float *)u, P.h = (u16 *)h;
-    gf_launch<EP_GLU, false, false>(P, s);
+    gf_launch_rows<EP_GLU, false>(P, s);
     GfParams Q{};
     Q.a = gf_mat((const u16 *)h, Fp, R, Fp), Q.b = gf_mat(pd, ldd, E, gf_up(F, 8));
-    Q.M = R, Q.N = E, Q.K = gf_up(F, 8), Q.nsplit = gf_splits(R, E, Q.K), Q.part = part, Q.bias0 = (const u16 *)bd, Q.F = Q.osplit = R, Q.out = (u16 *)y, Q.ldo = E;
-    gf_launch<EP_OUT, false, false>(Q, s);
+    Q.M = R, Q.N = E, Q.K = gf_up(F, 8), Q.nsplit = gf_splits(R, E, Q.K), Q.part = part, Q.bias0 = (const u16 *)bd, Q.out = (u16 *)y, Q.ldo = E;
+    gf_launch_rows<EP_OUT, false>(Q, s);
     GfClose c{};
     gf_join(c, Q);
     gf_close(c, s);
@@ -791,7 +839,7 @@ extern "C" int pcm_gated_ffn_backward_hip(long R, int E, int F, int act, const v
     char *at = (char *)ws + gf_up(R * 2 * Fp * 2, 256);
     float *sums = (float *)at;
     at += gf_sum_bytes(R, E, Fp);
-    float *const part_dx = (float *)at, *const part_w1 = part_dx + gf_part_bytes(R, E, 2 * Fp) / 4, *const part_w2 = part_w1 + gf_part_bytes(2 * Fp, E, R) / 4;
+    float *const part_dx = (float *)at, *const part_w1 = part_dx + gf_row_part_bytes(R, E, 2 * Fp) / 4, *const part_w2 = part_w1 + gf_part_bytes(2 * Fp, E, R) / 4;
     at += gf_back_part_bytes(R, E, F);
     GfClose c{};
     GfPacker pk(at, (char *)ws + ws_bytes - at);
@@ -806,13 +854,13 @@ extern "C" int pcm_gated_ffn_backward_hip(long R, int E, int F, int act, const v
         P.a = gf_mat(py, ldy, R, Ep), P.b = gf_mat(pd, ldd, E, gf_up(F, 8));
         P.M = R, P.N = Fp, P.K = Ep, P.act = act, P.nsplit = 1, P.F = F, P.Fp = Fp;
         P.out = dau, P.ka = (float *)a, P.ku = (float *)u, P.part = dbg ? sums : nullptr;
-        gf_launch<EP_DGLU, false, true>(P, s);
+        gf_launch_rows<EP_DGLU, true>(P, s);
     }
     if (dx) {
         GfParams P{};
         P.a = gf_mat(dau, 2 * Fp, R, 2 * Fp), P.b = gf_mat2(pg, pu, ldg, Fp, F, Ep);
-        P.M = R, P.N = E, P.K = 2 * Fp, P.nsplit = gf_splits(P.M, P.N, P.K), P.part = part_dx, P.F = P.osplit = R, P.out = (u16 *)dx, P.ldo = E;
-        gf_launch<EP_OUT, false, true>(P, s);
+        P.M = R, P.N = E, P.K = 2 * Fp, P.nsplit = gf_splits(P.M, P.N, P.K), P.part = part_dx, P.out = (u16 *)dx, P.ldo = E;
+        gf_launch_rows<EP_OUT, true>(P, s);
         gf_join(c, P);
     }
     if (dwg) {

@@ -155,3 +155,9 @@ def test_weights_of_different_alignment():
         g, u = buf[start:start + wg.numel()].view_as(wg), buf[start + wg.numel() + 3:][:wu.numel()].view_as(wu)
         g.copy_(wg), u.copy_(wu)
         assert torch.equal(gated_ffn(x.to(DEV), g, u, *(t.to(DEV) for t in (wd, bg, bu, bd))), want)
+
+
+@pytest.mark.parametrize("r,e,f", [(4120, 512, 2040), (4120, 2048, 520)])
+def test_rows_past_whole_rounds_at_size(r, e, f):
+    """24 rows more than whole rounds of tiles: a second launch for them (both projections and dh; y and dx, with split contractions)."""
+    _check(_inputs(r, e, f, True, seed=11), "gelu")
