@@ -187,14 +187,14 @@ def test_two_captured_graphs_share_nothing():
         f = lambda q=q, k=k, v=v, x=x, wg=wg, wu=wu, wd=wd: (cross_attention(q, k, v), gated_ffn(x, wg, wu, wd))  # noqa: E731
         want = f()
         graph, out = _graphs.captured(f)
-        sets.append((graph, out, want))
+        sets.append((graph, out, want, f))  # f: a graph reads its inputs where they were, they have to live as long
     streams = [torch.cuda.Stream() for _ in sets]
     for _ in range(5):
-        for st, (graph, _, _) in zip(streams, sets):
+        for st, (graph, *_) in zip(streams, sets):
             with torch.cuda.stream(st):
                 graph.replay()
         torch.cuda.synchronize()
-        for _, out, want in sets:
+        for _, out, want, _ in sets:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
