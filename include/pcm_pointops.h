@@ -688,9 +688,9 @@ int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, const void 
  * 16-byte aligned.  mask (nullable): bytes, != 0 = ignore the key; (B, S) at mask_bs, or (kv_rows) for a packed side.  out, dq:
  * (q rows, H, D) contiguous; dk, dv: (kv rows, Hkv, D) contiguous; lse (nullable in the forward), delta: (q rows, H) fp32.  A row without
  * a key: out = 0, lse = -inf, dq = 0.  Rows of a packed side behind the last sequence: 0 as well.  Offsets are clamped to the row count.
- * ws: pcm_cross_attn_ws_bytes bytes (0: none needed), 16-byte aligned, for either direction.  No atomics: results are reproducible. */
+ * ws: pcm_cross_attn_ws_bytes bytes (0: none needed), 16-byte aligned.  No atomics: results are reproducible. */
 int pcm_cross_attn_supported(int H, int Hkv, int D);
-long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed);
+long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, int backward);
 int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
                                const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
                                long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,

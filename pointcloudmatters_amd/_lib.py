@@ -156,7 +156,7 @@ SIGNATURES = {
     # B, L, H, D, x_is_bf16, x + 3 strides, out + 3 strides, coords_type, coords + 2 strides, axes, sections, base, interleaved, inverse, stream
     "pcm_rotary_axes_hip": [_l, _l, _i, _i, _i, _P, _l, _l, _l, _P, _l, _l, _l, _i, _P, _l, _l, _i, _P, ctypes.c_double, _i, _i, _P],
     "pcm_cross_attn_supported": [_i, _i, _i],
-    "pcm_cross_attn_ws_bytes": [_i, _i, _i, _i, _i, _l, _i, _i, _l, _i],
+    "pcm_cross_attn_ws_bytes": [_i, _i, _i, _i, _i, _l, _i, _i, _l, _i, _i],
     # B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset, (q, k, v) + 3 strides each, mask, mask_bs, scale, out, lse, ws, ws_bytes, stream
     "pcm_cross_attn_forward_hip": [_i, _i, _i, _i, _i, _l, _P, _i, _l, _P] + 3 * [_P, _l, _l, _l] + [_P, _l, _f, _P, _P, _P, _l, _P],
     # ..., scale, out, lse, dout + 3 strides, delta, dq, dk, dv, ws, ws_bytes, stream

@@ -480,16 +480,17 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_fwd_kernel(XaParams P)
     xa_finish<DP>(P, R, w.o, w.m, w.l, h);
 }
 
-// Few rows (up to 32 of a key head: one token of a rollout, a group of heads that share one): all four waves hold the same rows and share
-// the keys, wave w every fourth run of 32, each with LDS tiles and waits of its own (no barrier until the end).  K and V are read once and
-// nothing else is long, so what counts is requests in flight: two tiles of K and V a wave.  The waves' sums are joined through LDS.
-template <int DP>
-__global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
+// Few rows (up to 32 of a key head: one token of a rollout, a group of heads that share one): all waves hold the same rows and share
+// the keys, wave w every WAVES-th run of 32, each with LDS tiles and waits of its own (no barrier until the end).  K and V are read once and
+// nothing else is long, so what counts is requests in flight: two tiles of K and V a wave (128 KB for 8 waves and heads of 64, for
+// 4 and 128).  The waves' sums are joined through LDS.
+template <int DP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) pcm_xattn_few_kernel(XaParams P)
 {
-    constexpr int TILE = 32 * DP;
-    __shared__ __attribute__((aligned(1024))) u16 t0[4 * 2 * TILE], t1[4 * 2 * TILE];
-    __shared__ float sm[4][32], sl[4][32];
-    __shared__ __attribute__((aligned(16))) float bias[4][2][32];
+    constexpr int TILE = 32 * DP, STEP = 32 * WAVES;
+    __shared__ __attribute__((aligned(1024))) u16 t0[WAVES * 2 * TILE], t1[WAVES * 2 * TILE];
+    __shared__ float sm[WAVES][32], sl[WAVES][32];
+    __shared__ __attribute__((aligned(16))) float bias[WAVES][2][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     const XaLane<DP> ln(lane);
     XaRows R;
@@ -508,23 +509,23 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
         next = xa_visible(R.mask, mb, key0, R.ks.n, lane) & 0xFFFFFFFFull;
         if (next != 0xFFFFFFFFull && lane < 32) tb[lane] = xa_bias(next, lane);
         st.load(R.k, P.k_ls, key0, next, tk, 0), st.load(R.v, P.v_ls, key0, next, tk + TILE, 0);
-        mb = xa_mask_byte(R.mask, key0 + 128 + lane, R.ks.n);
+        mb = xa_mask_byte(R.mask, key0 + STEP + lane, R.ks.n);
     };
     const auto step = [&](int key0, int buf, const u16 *tk, u16 *nk) {
         __builtin_amdgcn_s_waitcnt(0x70);  // this wave's tile has arrived, its reads of the other are done
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         vis = next;
-        if (key0 + 128 < R.key_hi) request(key0 + 128, nk, bias[wave][1 - buf]);
+        if (key0 + STEP < R.key_hi) request(key0 + STEP, nk, bias[wave][1 - buf]);
         if (vis != 0) w.template tile<1>(tk, tk + TILE, qf, vis == 0xFFFFFFFFull, bias[wave][buf], c, ln, h);
     };
     int key0 = R.key_lo + 32 * wave;
     if (key0 < R.key_hi) {
         mb = xa_mask_byte(R.mask, key0 + lane, R.ks.n);
         request(key0, k0, bias[wave][0]);
-        for (; key0 + 128 < R.key_hi; key0 += 256) {
+        for (; key0 + STEP < R.key_hi; key0 += 2 * STEP) {
             step(key0, 0, k0, k1);
-            step(key0 + 128, 1, k1, k0);
+            step(key0 + STEP, 1, k1, k0);
         }
         if (key0 < R.key_hi) step(key0, 0, k0, k1);
     }
@@ -533,15 +534,15 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
     __syncthreads();
     float m = sm[0][col];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) m = fmaxf(m, sm[i][col]);
+    for (int i = 1; i < WAVES; ++i) m = fmaxf(m, sm[i][col]);
     float l = 0.f, mine = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
         const float f = sl[i][col] == 0.f ? 0.f : __builtin_amdgcn_exp2f((sm[i][col] - m) * c);
         if (sl[i][col] != 0.f) l = __builtin_fmaf(sl[i][col], f, l);
         if (i == wave) mine = f;
     }
-    // O^T of the waves, one after the other in wave order: [register][lane] in the tiles' memory (4 * DP * 2 bytes a lane fit)
+    // O^T of the waves, one after the other in wave order: [register][lane] in the first tiles' memory
     float *const sum = (float *)t0;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(256) pcm_xattn_few_kernel(XaParams P)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int k = 0; k < 3; ++k) w.o[i][r] += sum[(k * (DP / 2) + 16 * i + r) * 64 + lane];
+            for (int k = 0; k < WAVES - 1; ++k) w.o[i][r] += sum[(k * (DP / 2) + 16 * i + r) * 64 + lane];
     xa_finish<DP>(P, R, w.o, m, l, h);
 }
 
@@ -957,23 +958,29 @@ long xa_tiles(int packed, int B, int len, long rows, int mult, int per)
 // sequence is not known here: only its total counts.
 bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows : (long)L) * G <= 32; }
 
-// Splits of the keys.  A workgroup per (tile, key head) is too few for 256 compute units when the rows are few (one token of a rollout,
-// a decoder's 100 queries): the keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and
-// re-reads its row's fp32 sums and costs a second launch (4 - 5 us), so it has 256 keys at least (for one row over 2051 keys, 8 heads: 10 us
-// with 8 splits, 20 with one).  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave
-// hides the others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 255 us with one split, 192 + 10
-// for the joining with four).
-int xa_splits(int B, int H, int Hkv, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed)
+// Splits of the keys.  A workgroup per (tile, key head) is too few for 256 compute units when the rows are few (a decoder's 100 queries): the
+// keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and re-reads its row's fp32 sums and costs a
+// second launch (4 - 7 us), so it has 256 keys at least.  The kernel of few rows shares the keys among its own waves (8, or 4 for heads wider
+// than 64) and splits only past 256 keys for each of them: one row over 2051 keys, 8 heads of 64, takes 13.4 us without a split and
+// 10.4 + 4.8 with 7.  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave hides the
+// others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 255 us with one split where four
+// took 192 + 10 for the joining).
+int xa_splits(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, bool backward)
 {
     const int G = H / Hkv;
+    const bool few = !backward && xa_few(L, q_rows, q_packed, G);
     const long work = (q_packed ? (q_rows * G + XA_ROWS - 1) / XA_ROWS + B - 1 : xa_tiles(0, B, L, q_rows, G, XA_ROWS)) * Hkv;
     const long keys = kv_packed ? (kv_rows + B - 1) / B : S, w = work > 0 ? work : 1;
-    long n = 512 / w < keys / 256 ? 512 / w : keys / 256;
+    const long least = few ? (D <= 64 ? 2048 : 1024) : 256;
+    long n = 512 / w < keys / least ? 512 / w : keys / least;
     const long more = 1536 / w < keys / 2048 ? 1536 / w : keys / 2048;
     n = n > more ? n : more;
     return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
-int xa_splits(const XaParams &P) { return xa_splits(P.B, P.H, P.Hkv, P.L, P.q_rows, P.q_off != nullptr, P.S, P.kv_rows, P.kv_off != nullptr); }
+int xa_splits(const XaParams &P, bool backward)
+{
+    return xa_splits(P.B, P.H, P.Hkv, P.D, P.L, P.q_rows, P.q_off != nullptr, P.S, P.kv_rows, P.kv_off != nullptr, backward);
+}
 
 // Splits of the rows for dK and dV, where few keys leave compute units idle: at least 512 rows (8 tiles) each.
 int xa_row_splits(int B, int Hkv, int G, long q_rows, int S, long kv_rows, int kv_packed)
@@ -1024,12 +1031,14 @@ unsigned xa_grid(long items) { return (unsigned)((items + 7) / 8 * 8); }
 
 extern "C" int pcm_cross_attn_supported(int H, int Hkv, int D) { return xa_shape_ok(H, Hkv, D) ? 1 : 0; }
 
-extern "C" long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed)
+extern "C" long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed,
+                                        int backward)
 {
     if (B <= 0 || L < 0 || S < 0 || q_rows < 0 || kv_rows < 0 || !xa_shape_ok(H, Hkv, D)) return 0;
     if (!q_packed) q_rows = (long)B * L;
     if (!kv_packed) kv_rows = (long)B * S;
-    const int n = xa_splits(B, H, Hkv, L, q_rows, q_packed, S, kv_rows, kv_packed), m = xa_row_splits(B, Hkv, H / Hkv, q_rows, S, kv_rows, kv_packed);
+    const int n = xa_splits(B, H, Hkv, D, L, q_rows, q_packed, S, kv_rows, kv_packed, backward != 0);
+    const int m = backward ? xa_row_splits(B, Hkv, H / Hkv, q_rows, S, kv_rows, kv_packed) : 1;
     const long rows = n > 1 ? (long)n * q_rows * H * (D + 2) * 4 : 0, keys = m > 1 ? (long)m * 2 * kv_rows * Hkv * D * 4 : 0;
     return rows > keys ? rows : keys;
 }
@@ -1048,14 +1057,17 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     if (!out || (((uintptr_t)out | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
     P.out = (u16 *)out, P.lse = lse;
     const bool few = xa_few(L, P.q_rows, q_offset != nullptr, P.G);
-    P.nsplit = xa_splits(P);
+    P.nsplit = xa_splits(P, false);
     if (P.nsplit > 1) {
         if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * (D + 2) * 4) return PCM_ERR_BAD_ARG;
         P.part_o = (float *)ws, P.part_ml = (float *)ws + (long)P.nsplit * P.q_rows * H * D;
     }
     P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS), P.each = q_offset ? 1 : P.tiles / B;
     const hipStream_t s = (hipStream_t)stream;
-    if (few) XA_BY_DIM(pcm_xattn_few_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
+    const dim3 grid(xa_grid((long)P.tiles * Hkv * P.nsplit));
+    if (few && D <= 32) hipLaunchKernelGGL((pcm_xattn_few_kernel<32, 8>), grid, dim3(512), 0, s, P);
+    else if (few && D <= 64) hipLaunchKernelGGL((pcm_xattn_few_kernel<64, 8>), grid, dim3(512), 0, s, P);
+    else if (few) hipLaunchKernelGGL((pcm_xattn_few_kernel<128, 4>), grid, dim3(256), 0, s, P);
     else XA_BY_DIM(pcm_xattn_fwd_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
     if (P.nsplit > 1) {
         const long rows = P.q_rows * H;
@@ -1086,7 +1098,7 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
     P.delta = delta, P.dq = (u16 *)dq, P.dk = (u16 *)dk, P.dv = (u16 *)dv;
     const hipStream_t s = (hipStream_t)stream;
     if (P.q_rows > 0) {
-        P.nsplit = xa_splits(P);
+        P.nsplit = xa_splits(P, true);
         if (P.nsplit > 1) {
             if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * D * 4) return PCM_ERR_BAD_ARG;
             P.part_o = (float *)ws;

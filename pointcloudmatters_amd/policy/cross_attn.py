@@ -35,8 +35,8 @@ def _new(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _arguments(q, k, v, mask, q_offset, kv_offset, scale):
-    """The operands as the kernels take them, the arguments that describe them, and the bytes of workspace of either direction."""
+def _arguments(q, k, v, mask, q_offset, kv_offset, scale, backward):
+    """The operands as the kernels take them, the arguments that describe them, and the bytes of workspace."""
     qshape, kshape = q.shape, k.shape
     (q, qs), (k, ks), (v, vs) = _fit(q, qshape[-2] // kshape[-2]), _fit(k), _fit(v)
     h, d, hkv = qshape[-2], qshape[-1], kshape[-2]
@@ -44,13 +44,13 @@ def _arguments(q, k, v, mask, q_offset, kv_offset, scale):
     s, kv_rows, ko = (kshape[1], kshape[0] * kshape[1], 0) if len(kshape) == 4 else (0, kshape[0], kv_offset.data_ptr())
     args = (b, h, hkv, d, l, q_rows, qo, s, kv_rows, ko, q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
             mask.data_ptr() if mask is not None else 0, s, scale)
-    return q, k, v, args, _lib.load().pcm_cross_attn_ws_bytes(b, h, hkv, d, l, q_rows, qo != 0, s, kv_rows, ko != 0)
+    return q, k, v, args, _lib.load().pcm_cross_attn_ws_bytes(b, h, hkv, d, l, q_rows, qo != 0, s, kv_rows, ko != 0, backward)
 
 
 def _forward(q, k, v, mask, q_offset, kv_offset, scale, want_lse):
     dev = q.device
     with _lib.on_device(dev):
-        q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, scale)
+        q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, scale, False)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         out = _new(q)
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
@@ -79,7 +79,7 @@ def _backward(ctx, dout):
     q, k, v, mask, q_offset, kv_offset, out, lse = ctx.saved_tensors
     dev = q.device
     with _lib.on_device(dev):
-        q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale)
+        q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale, True)
         dout, gs = _fit(dout, q.shape[-2] // k.shape[-2])
         dq, dk, dv = _new(q), _new(k), _new(v)
         at = lse.numel() * 4 + 15 & ~15

@@ -154,7 +154,7 @@ def test_entry_points_reject_before_they_touch_the_runtime():
         assert xa(S=0x7FFFFF00, back=back) == 2 and xa(H=1 << 10, Hkv=1 << 10, S=0x7FFFF000, back=back) == 2  # more threads than a launch takes
         assert xa(S=100000, back=back) == 1  # split keys need their workspace
     assert L.pcm_cross_attn_supported(8, 2, 64) == 1 and L.pcm_cross_attn_supported(8, 3, 64) == 0 and L.pcm_cross_attn_supported(8, 2, 4) == 0
-    assert L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 5, 5, 0) == 0 < L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 100000, 100000, 0)
+    assert L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 5, 5, 0, 0) == 0 < L.pcm_cross_attn_ws_bytes(1, 2, 1, 64, 3, 3, 0, 100000, 100000, 0, 0)
 
     def ff(R=40, E=16, F=8, act=0, x=p, a=None, u=None, h=p, ws=p, wsb=1 << 30):
         return L.pcm_gated_ffn_forward_hip(R, E, F, act, x, E, p, p, p, None, None, None, p, a, u, h, ws, wsb, None)
