@@ -686,7 +686,8 @@ int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, const void 
  * Each side is padded (offset NULL: B sequences of L resp. S rows at the batch stride) or packed (offset: B cumulative ends on the
  * device; q_rows resp. kv_rows = all rows; the batch stride is ignored).  Strides (bs, ls, hs) in elements, multiples of 8; pointers
  * 16-byte aligned.  mask (nullable): bytes, != 0 = ignore the key; (B, S) at mask_bs, or (kv_rows) for a packed side.  out, dq:
- * (q rows, H, D) contiguous; dk, dv: (kv rows, Hkv, D) contiguous; lse (nullable in the forward), delta: (q rows, H) fp32.  A row without
+ * (q rows, H, D) contiguous; dk, dv: (kv rows, Hkv, D) contiguous; out32 (out in fp32) and lse, both for the backward,
+ * nullable in the forward; lse, delta: (q rows, H) fp32.  A row without
  * a key: out = 0, lse = -inf, dq = 0.  Rows of a packed side behind the last sequence: 0 as well.  Offsets are clamped to the row count.
  * ws: pcm_cross_attn_ws_bytes bytes (0: none needed), 16-byte aligned.  No atomics: results are reproducible. */
 int pcm_cross_attn_supported(int H, int Hkv, int D);
@@ -694,11 +695,11 @@ long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, long q_rows, i
 int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
                                const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
                                long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,
-                               long mask_bs, float scale, void *out, float *lse, void *ws, long ws_bytes, void *stream);
+                               long mask_bs, float scale, void *out, float *out32, float *lse, void *ws, long ws_bytes, void *stream);
 int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
                                 const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
                                 long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,
-                                long mask_bs, float scale, const void *out, const float *lse, const void *dout, long g_bs, long g_ls,
+                                long mask_bs, float scale, const float *out32, const float *lse, const void *dout, long g_bs, long g_ls,
                                 long g_hs, float *delta, void *dq, void *dk, void *dv, void *ws, long ws_bytes, void *stream);
 
 /* ---- gated feed-forward block (csrc/gated_ffn.hip) ------------------------------------------------------------------

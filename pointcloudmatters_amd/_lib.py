@@ -157,9 +157,9 @@ SIGNATURES = {
     "pcm_rotary_axes_hip": [_l, _l, _i, _i, _i, _P, _l, _l, _l, _P, _l, _l, _l, _i, _P, _l, _l, _i, _P, ctypes.c_double, _i, _i, _P],
     "pcm_cross_attn_supported": [_i, _i, _i],
     "pcm_cross_attn_ws_bytes": [_i, _i, _i, _i, _i, _l, _i, _i, _l, _i, _i],
-    # B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset, (q, k, v) + 3 strides each, mask, mask_bs, scale, out, lse, ws, ws_bytes, stream
-    "pcm_cross_attn_forward_hip": [_i, _i, _i, _i, _i, _l, _P, _i, _l, _P] + 3 * [_P, _l, _l, _l] + [_P, _l, _f, _P, _P, _P, _l, _P],
-    # ..., scale, out, lse, dout + 3 strides, delta, dq, dk, dv, ws, ws_bytes, stream
+    # B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset, (q, k, v) + 3 strides each, mask, mask_bs, scale, out, out32, lse, ws, ws_bytes, stream
+    "pcm_cross_attn_forward_hip": [_i, _i, _i, _i, _i, _l, _P, _i, _l, _P] + 3 * [_P, _l, _l, _l] + [_P, _l, _f, _P, _P, _P, _P, _l, _P],
+    # ..., scale, out32, lse, dout + 3 strides, delta, dq, dk, dv, ws, ws_bytes, stream
     "pcm_cross_attn_backward_hip": [_i, _i, _i, _i, _i, _l, _P, _i, _l, _P] + 3 * [_P, _l, _l, _l] + [_P, _l, _f, _P, _P, _P, _l, _l, _l]
     + 5 * [_P] + [_l, _P],
     "pcm_gated_ffn_hidden_ld": [_i],

@@ -18,8 +18,8 @@
 //
 // Masked or absent keys are zeroed in K and V where a tile is staged (a NaN or infinity in padding must not meet a zero weight) and
 // their scores start from -inf.  Sums, maxima, lse, delta and accumulators are fp32; P and dS are rounded to bf16 (one half step,
-// 2^-8 relative at most) because the matrix operands are bf16; outputs are rounded once; delta reads O as it was stored (its rounding's
-// part of dQ is a fraction of dS's own: O is an average of V).
+// 2^-8 relative at most) because the matrix operands are bf16; outputs are rounded once.  For delta O is
+// kept in fp32 beside lse: over few keys a rounded O took dQ and dK from 2.4e-3 of their norm to 2.9e-3.
 #include "pcm_attn.hpp"
 
 namespace {
@@ -39,7 +39,7 @@ struct XaParams {
     float scale;
     int tiles, each, nsplit;  // each: tiles of a padded sequence
     u16 *out, *dq, *dk, *dv;
-    float *lse, *delta, *part_o, *part_ml;
+    float *o32, *lse, *delta, *part_o, *part_ml;
     // row / G by one multiplication: g_inv = 2^g_shift / G rounded up, 2^(g_shift - 31) >= G.  g_inv * G exceeds 2^g_shift by less than G,
     // so the product is off by less than row * G <= 2^31 * 2^(g_shift - 31) of 2^g_shift: exact for every row below 2^31
     uint32_t g_inv;
@@ -425,7 +425,10 @@ __device__ __forceinline__ void xa_finish(const XaParams &P, const XaRows &R, co
     const float inv = l == 0.f ? 0.f : 1.f / l;  // l >= 1 with a key (its largest weight is 1), NaN with a NaN among the scores
     if (P.lse && h == 0) P.lse[R.out_row] = l == 0.f ? -INFINITY : m * P.scale + __logf(l);
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) xa_store_row(P.out + R.out_row * P.D, P.D, h, i, o[i], inv);
+    for (int i = 0; i < DP / 32; ++i) {
+        xa_store_row(P.out + R.out_row * P.D, P.D, h, i, o[i], inv);
+        if (P.o32) xa_store_part(P.o32 + R.out_row * P.D, P.D, h, i, o[i] * inv);
+    }
 }
 
 // The keys of a row kernel, 64 at a time through two LDS buffers of K and V: while tile t is worked on, tile t + 1 is on its way.  The
@@ -590,7 +593,9 @@ __global__ void __launch_bounds__(256) pcm_xattn_join_kernel(XaParams P)
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (P.lse && d == 0) P.lse[row] = l == 0.f ? -INFINITY : m * P.scale + __logf(l);
-        *(uint2 *)(P.out + row * P.D + d) = make_uint2(cvt_pk_bf16(o.x * inv, o.y * inv), cvt_pk_bf16(o.z * inv, o.w * inv));
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        *(uint2 *)(P.out + row * P.D + d) = make_uint2(cvt_pk_bf16(o.x, o.y), cvt_pk_bf16(o.z, o.w));
+        if (P.o32) *(float4 *)(P.o32 + row * P.D + d) = o;
     }
 }
 
@@ -607,13 +612,16 @@ __global__ void __launch_bounds__(256, 2) pcm_xattn_dq_kernel(XaParams P)
     bf8 qf[DP / 16], gf[DP / 16];
     float delta = 0.f;
     {
-        bf8 of[DP / 16];
-        xa_row_operand<DP>(P.out + R.out_row * P.D, R.ok, P.D, h, of);
         xa_row_operand<DP>(xa_q_row(P, P.dout, P.g_bs, P.g_ls, P.g_hs, R), R.ok, P.D, h, gf);
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t)
+        for (int t = 0; t < DP / 16; ++t) {
+            if (!R.ok || 16 * t + 8 * h >= P.D) continue;
+            const float *const row = P.o32 + R.out_row * P.D + 16 * t + 8 * h;
+            const float4 a = *(const float4 *)row, b = *(const float4 *)(row + 4);
+            const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)of[t][e], (float)gf[t][e], delta);
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(f[e], (float)gf[t][e], delta);
+        }
         delta += __shfl_xor(delta, 32);
     }
     xa_row_operand<DP>(xa_q_row(P, P.q, P.q_bs, P.q_ls, P.q_hs, R), R.ok, P.D, h, qf);
@@ -1046,7 +1054,7 @@ extern "C" long pcm_cross_attn_ws_bytes(int B, int H, int Hkv, int D, int L, lon
 extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
                                           const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
                                           long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,
-                                          long mask_bs, float scale, void *out, float *lse, void *ws, long ws_bytes, void *stream)
+                                          long mask_bs, float scale, void *out, float *out32, float *lse, void *ws, long ws_bytes, void *stream)
 {
     if (B < 0 || H < 0 || Hkv < 0 || D < 0 || L < 0 || S < 0 || q_rows < 0 || kv_rows < 0) return PCM_ERR_BAD_ARG;
     if (B == 0 || (q_offset ? q_rows == 0 : L == 0)) return PCM_OK;
@@ -1054,8 +1062,8 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     const int bad = xa_fill(P, B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset, q, q_bs, q_ls, q_hs, k, k_bs, k_ls, k_hs, v, v_bs, v_ls, v_hs,
                             mask, mask_bs, scale);
     if (bad) return bad;
-    if (!out || (((uintptr_t)out | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
-    P.out = (u16 *)out, P.lse = lse;
+    if (!out || (((uintptr_t)out | (uintptr_t)out32 | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
+    P.out = (u16 *)out, P.o32 = out32, P.lse = lse;
     const bool few = xa_few(L, P.q_rows, q_offset != nullptr, P.G);
     P.nsplit = xa_splits(P, false);
     if (P.nsplit > 1) {
@@ -1081,7 +1089,7 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
 extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, long q_rows, const int *q_offset, int S, long kv_rows,
                                            const int *kv_offset, const void *q, long q_bs, long q_ls, long q_hs, const void *k, long k_bs,
                                            long k_ls, long k_hs, const void *v, long v_bs, long v_ls, long v_hs, const unsigned char *mask,
-                                           long mask_bs, float scale, const void *out, const float *lse, const void *dout, long g_bs, long g_ls,
+                                           long mask_bs, float scale, const float *out32, const float *lse, const void *dout, long g_bs, long g_ls,
                                            long g_hs, float *delta, void *dq, void *dk, void *dv, void *ws, long ws_bytes, void *stream)
 {
     if (B < 0 || H < 0 || Hkv < 0 || D < 0 || L < 0 || S < 0 || q_rows < 0 || kv_rows < 0) return PCM_ERR_BAD_ARG;
@@ -1090,11 +1098,11 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
     const int bad = xa_fill(P, B, H, Hkv, D, L, q_rows, q_offset, S, kv_rows, kv_offset, q, q_bs, q_ls, q_hs, k, k_bs, k_ls, k_hs, v, v_bs, v_ls, v_hs,
                             mask, mask_bs, scale);
     if (bad) return bad;
-    if (P.q_rows > 0 && (!out || !lse || !dout || !delta || !dq)) return PCM_ERR_BAD_ARG;
+    if (P.q_rows > 0 && (!out32 || !lse || !dout || !delta || !dq)) return PCM_ERR_BAD_ARG;
     if (P.kv_rows > 0 && (!dk || !dv)) return PCM_ERR_BAD_ARG;
     if (!xa_strides_ok(dout, g_bs, g_ls, g_hs, H / Hkv)) return PCM_ERR_UNSUPPORTED;
-    if ((((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
-    P.out = (u16 *)out, P.lse = (float *)lse, P.dout = (const u16 *)dout, P.g_bs = g_bs, P.g_ls = g_ls, P.g_hs = g_hs;
+    if ((((uintptr_t)out32 | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
+    P.o32 = (float *)out32, P.lse = (float *)lse, P.dout = (const u16 *)dout, P.g_bs = g_bs, P.g_ls = g_ls, P.g_hs = g_hs;
     P.delta = delta, P.dq = (u16 *)dq, P.dk = (u16 *)dk, P.dv = (u16 *)dv;
     const hipStream_t s = (hipStream_t)stream;
     if (P.q_rows > 0) {

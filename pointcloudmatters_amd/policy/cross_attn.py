@@ -47,26 +47,28 @@ def _arguments(q, k, v, mask, q_offset, kv_offset, scale, backward):
     return q, k, v, args, _lib.load().pcm_cross_attn_ws_bytes(b, h, hkv, d, l, q_rows, qo != 0, s, kv_rows, ko != 0, backward)
 
 
-def _forward(q, k, v, mask, q_offset, kv_offset, scale, want_lse):
+def _forward(q, k, v, mask, q_offset, kv_offset, scale, want_lse, keep):
+    """out, its fp32 form for a backward pass (keep), lse, and the operands as the kernels took them."""
     dev = q.device
     with _lib.on_device(dev):
         q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, scale, False)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         out = _new(q)
+        out32 = torch.empty(q.shape, dtype=torch.float32, device=dev) if keep else None
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
-        rc = _lib.load().pcm_cross_attn_forward_hip(*args, out.data_ptr(), lse.data_ptr() if want_lse else 0, ws.data_ptr() if ws_bytes else 0,
-                                                    ws_bytes, _raw_stream())
+        rc = _lib.load().pcm_cross_attn_forward_hip(*args, out.data_ptr(), out32.data_ptr() if keep else 0, lse.data_ptr() if want_lse else 0,
+                                                    ws.data_ptr() if ws_bytes else 0, ws_bytes, _raw_stream())
     if rc:
         _lib.check(rc, "pcm_cross_attn_forward_hip")
-    return out, lse, q, k, v
+    return out, out32, lse, q, k, v
 
 
 class _CrossAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, q_offset, kv_offset, scale):
-        out, lse, q, k, v = _forward(q, k, v, mask, q_offset, kv_offset, scale, True)
+        out, out32, lse, q, k, v = _forward(q, k, v, mask, q_offset, kv_offset, scale, True, True)
         ctx.mark_non_differentiable(lse)
-        ctx.save_for_backward(q, k, v, mask, q_offset, kv_offset, out, lse)
+        ctx.save_for_backward(q, k, v, mask, q_offset, kv_offset, out32, lse)
         ctx.scale = scale
         return out, lse
 
@@ -76,7 +78,7 @@ class _CrossAttention(Function):
 
 
 def _backward(ctx, dout):
-    q, k, v, mask, q_offset, kv_offset, out, lse = ctx.saved_tensors
+    q, k, v, mask, q_offset, kv_offset, out32, lse = ctx.saved_tensors
     dev = q.device
     with _lib.on_device(dev):
         q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale, True)
@@ -85,7 +87,7 @@ def _backward(ctx, dout):
         at = lse.numel() * 4 + 15 & ~15
         ws = torch.empty(at + ws_bytes, dtype=torch.uint8, device=dev)  # delta, then the workspace
         p = ws.data_ptr()
-        rc = _lib.load().pcm_cross_attn_backward_hip(*args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), *gs, p, dq.data_ptr(),
+        rc = _lib.load().pcm_cross_attn_backward_hip(*args, out32.data_ptr(), lse.data_ptr(), dout.data_ptr(), *gs, p, dq.data_ptr(),
                                                      dk.data_ptr(), dv.data_ptr(), p + at, ws_bytes, _raw_stream())
     if rc:
         _lib.check(rc, "pcm_cross_attn_backward_hip")
@@ -148,5 +150,5 @@ def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=Non
         out, lse = _CrossAttention.apply(q, k, v, mask, q_offset, kv_offset, scale)
         _graphs.guard_leaves(out, "cross_attention")
     else:
-        out, lse, *_ = _forward(q, k, v, mask, q_offset, kv_offset, scale, return_lse)
+        out, _, lse, *_ = _forward(q, k, v, mask, q_offset, kv_offset, scale, return_lse, False)
     return (out, lse) if return_lse else out

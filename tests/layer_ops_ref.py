@@ -81,7 +81,7 @@ def attention(q, k, v, mask, q_spans, k_spans, scale, dout=None):
             dp = G @ V.T
             delta = (G * o).sum(-1, keepdim=True)
             edp = (D + 4) * F32 * (G.abs() @ V.abs().T)
-            # delta reads the output as it was stored
+            # delta from the output as it was stored, at worst (kept in fp32 it is closer)
             ed = (G.abs() * (eoo + HALF * (o.abs() + eoo))).sum(-1, keepdim=True) + (D + 4) * F32 * (G.abs() * o.abs()).sum(-1, keepdim=True)
             ds = p * (dp - delta)
             # weights recomputed from lse: its error once more

@@ -145,7 +145,7 @@ def test_entry_points_reject_before_they_touch_the_runtime():
         head = (1, H, Hkv, D, 3, 3, None, S, kv_rows, None, q, 0, q_ls, 64, p, 0, 64, 64, p, 0, 64, 64, None, 0, scale)
         if back:
             return L.pcm_cross_attn_backward_hip(*head, out, p, p, 0, 128, 64, p, p, p, p, ws, wsb, None)
-        return L.pcm_cross_attn_forward_hip(*head, out, p, ws, wsb, None)
+        return L.pcm_cross_attn_forward_hip(*head, out, p, p, ws, wsb, None)
 
     for back in (False, True):
         assert xa(H=3, Hkv=2, back=back) == 2 and xa(D=60, back=back) == 2 and xa(D=136, back=back) == 2 and xa(q_ls=129, back=back) == 2
