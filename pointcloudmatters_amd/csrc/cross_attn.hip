@@ -259,11 +259,16 @@ struct XaLane {
 // use and waits out the whole LDS latency each time; with one or two waves a SIMD that was most of the time of a tile.
 __device__ __forceinline__ void xa_keep() { __builtin_amdgcn_sched_barrier(0x406); }
 
+// A wave among matrix instructions goes before one among exponentials: the matrix cores are fed while others calculate weights (forward pass:
+// 171 and 166 us over a scene's 12000 keys, heads of 128 39 and 36 us).
+#define xa_matrix(on) __builtin_amdgcn_s_setprio(on)
+
 // acc[j] += A_j B_j over the DP channels, for N products: the operands of the next 16 channels are read before the present ones are multiplied
 template <int DP, int N, class FA, class FB>
 __device__ __forceinline__ void xa_products(f16v (&acc)[N], FA a, FB b)
 {
     bf8 x[2][N], y[2][N];
+    xa_matrix(1);
 #pragma unroll
     for (int j = 0; j < N; ++j) x[0][j] = a(j, 0), y[0][j] = b(j, 0);
 #pragma unroll
@@ -277,6 +282,7 @@ __device__ __forceinline__ void xa_products(f16v (&acc)[N], FA a, FB b)
         for (int j = 0; j < N; ++j) acc[j] = PCM_MFMA16(x[t & 1][j], y[t & 1][j], acc[j]);
         xa_keep();
     }
+    xa_matrix(0);
 }
 
 __device__ __forceinline__ unsigned xa_mask_byte(const unsigned char *m, int key, int n) { return m != nullptr && key < n ? (unsigned)m[key] : 0u; }
@@ -395,6 +401,7 @@ struct XaSoftmax {
                 sum += s[j][r];
             }
         l += sum;
+        xa_matrix(1);
 #pragma unroll
         for (int t = 0; t < 2 * NJ; ++t) {
             if (t + 1 < 2 * NJ) {
@@ -407,6 +414,7 @@ struct XaSoftmax {
             for (int i = 0; i < DP / 32; ++i) o[i] = PCM_MFMA16(vt[t & 1][i], p, o[i]);
             xa_keep();
         }
+        xa_matrix(0);
     }
 };
 
@@ -823,7 +831,7 @@ __device__ __forceinline__ void xa_store_keys(const XaParams &P, const XaKeys &K
 
 // dK and dV of 128 keys, heads wider than 64.  8 waves: four groups of 32 keys times the two halves of every 64-row tile of Q and dO, whose sums
 // are added at the end.  K and V stand in LDS beside the two buffers of Q and dO (128 KB): held in registers, as operands of 4 waves,
-// they left one wave a SIMD, which waited for its own LDS reads and exponentials (515 x 4 rows over 1027 keys: 119 us, now 88).
+// they left one wave a SIMD, which waited for its own LDS reads and exponentials (515 x 4 rows over 1027 keys: 119 us, now 74).
 // nsplit > 1: the rows are shared out and each share writes fp32 sums.
 template <int DP>
 __global__ void __launch_bounds__(512, 2) pcm_xattn_dkv_wide_kernel(XaParams P)
@@ -971,8 +979,8 @@ bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows
 // second launch (4 - 7 us), so it has 256 keys at least.  The kernel of few rows shares the keys among its own waves (8, or 4 for heads wider
 // than 64) and splits only past 256 keys for each of them: one row over 2051 keys, 8 heads of 64, takes 13.4 us without a split and
 // 10.4 + 4.8 with 7.  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave hides the
-// others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 255 us with one split where four
-// took 192 + 10 for the joining).
+// others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 230 us with one split, 173 + 7
+// for the joining with two, 167 + 10 with four).
 int xa_splits(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, bool backward)
 {
     const int G = H / Hkv;

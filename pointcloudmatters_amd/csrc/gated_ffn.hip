@@ -10,7 +10,7 @@
 // the same 32 of the up projection, so act(a) * u needs no exchange -- and so do dh, da and du.  h, da and du are rounded to bf16
 // where they are stored as operands of the next product (one half step, 2^-8 relative at most); outputs are rounded once.  a and u, of which
 // the backward pass forms da and du, are kept in fp32: as bf16 they brought dx, the weight and the bias gradients from 2.3e-3 of their norm
-// (the roundings of da, du and the output) to 3.0e-3, for 5 % less time (16408 rows, 512 -> 2048: 613 and 646 us forward and backward).
+// (the roundings of da, du and the output) to 3.0e-3, for 5 % less time (16408 rows, 512 -> 2048, forward and backward).
 //
 // a, u, h have rows of Fp = F rounded up to 64 values; the columns from F on are zero, so contractions over F need no edge.  Matrices
 // whose rows do not start at 16-byte boundaries (an odd width) are copied into padded rows first, one launch for all of a call's.
@@ -653,7 +653,8 @@ GfShape gf_shape(long M, long N, long K, int nsplit, bool wgrad)
 // Rows of a product's first launch.  Tiles a little over whole rounds of workgroups (one / two / three a compute unit) leave the last round nearly
 // empty: 16408 rows are 64 row tiles of 256 and 24 rows, 4 rounds and 16 tiles of a fifth.  Where the last round has under a third of a round's
 // tiles and a round is worth the launch (2^24 products a compute unit, some 20 us), its rows are multiplied by a second launch, in smaller tiles
-// and shared-out contractions of its own choice (16408 rows of 512 -> 2048, forward and backward: @@).
+// and shared-out contractions of its own choice (16408 rows of 512 -> 2048, forward and backward: 602 us, 633 with one launch a
+// product).
 long gf_first_rows(long M, long N, long K)
 {
     const GfShape t = gf_shape(M, N, K, 1, false);
