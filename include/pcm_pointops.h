@@ -686,7 +686,7 @@ int pcm_rotary_axes_hip(long B, long L, int H, int D, int x_is_bf16, const void 
  * Each side is padded (offset NULL: B sequences of L resp. S rows at the batch stride) or packed (offset: B cumulative ends on the
  * device; q_rows resp. kv_rows = all rows; the batch stride is ignored).  Strides (bs, ls, hs) in elements, multiples of 8; pointers
  * 16-byte aligned.  mask (nullable): bytes, != 0 = ignore the key; (B, S) at mask_bs, or (kv_rows) for a packed side.  out, dq:
- * (q rows, H, D) contiguous; dk, dv: (kv rows, Hkv, D) contiguous; out32 (out in fp32) and lse, both for the backward,
+ * (q rows, H, D) contiguous; dk, dv: (kv rows, Hkv, D) contiguous, both or neither; out32 (out in fp32) and lse, both for the backward,
  * nullable in the forward; lse, delta: (q rows, H) fp32.  A row without
  * a key: out = 0, lse = -inf, dq = 0.  Rows of a packed side behind the last sequence: 0 as well.  Offsets are clamped to the row count.
  * ws: pcm_cross_attn_ws_bytes bytes (0: none needed), 16-byte aligned.  No atomics: results are reproducible. */

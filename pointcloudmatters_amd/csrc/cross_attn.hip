@@ -1107,7 +1107,7 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
                             mask, mask_bs, scale);
     if (bad) return bad;
     if (P.q_rows > 0 && (!out32 || !lse || !dout || !delta || !dq)) return PCM_ERR_BAD_ARG;
-    if (P.kv_rows > 0 && (!dk || !dv)) return PCM_ERR_BAD_ARG;
+    if (!dk != !dv) return PCM_ERR_BAD_ARG;  // neither: states that need no gradient
     if (!xa_strides_ok(dout, g_bs, g_ls, g_hs, H / Hkv)) return PCM_ERR_UNSUPPORTED;
     if ((((uintptr_t)out32 | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
     P.o32 = (float *)out32, P.lse = (float *)lse, P.dout = (const u16 *)dout, P.g_bs = g_bs, P.g_ls = g_ls, P.g_hs = g_hs;
@@ -1123,7 +1123,7 @@ extern "C" int pcm_cross_attn_backward_hip(int B, int H, int Hkv, int D, int L, 
         XA_BY_DIM(pcm_xattn_dq_kernel, 256, xa_grid((long)P.tiles * Hkv * P.nsplit), s, P);
         if (P.nsplit > 1) hipLaunchKernelGGL(pcm_xattn_dq_join_kernel, dim3((unsigned)((P.q_rows * H * (D / 4) + 255) / 256)), dim3(256), 0, s, P);
     }
-    if (P.kv_rows > 0) {
+    if (P.kv_rows > 0 && dk) {
         P.tiles = (int)xa_tiles(kv_offset != nullptr, B, S, P.kv_rows, 1, XA_ROWS), P.each = kv_offset ? 1 : P.tiles / B;
         P.nsplit = xa_row_splits(P);
         if (P.nsplit > 1) {

@@ -83,15 +83,17 @@ def _backward(ctx, dout):
     with _lib.on_device(dev):
         q, k, v, args, ws_bytes = _arguments(q, k, v, mask, q_offset, kv_offset, ctx.scale, True)
         dout, gs = _fit(dout, q.shape[-2] // k.shape[-2])
-        dq, dk, dv = _new(q), _new(k), _new(v)
+        _, need_k, need_v, *_ = ctx.needs_input_grad
+        dq, dk, dv = _new(q), *((_new(k), _new(v)) if need_k or need_v else (None, None))
         at = lse.numel() * 4 + 15 & ~15
         ws = torch.empty(at + ws_bytes, dtype=torch.uint8, device=dev)  # delta, then the workspace
         p = ws.data_ptr()
         rc = _lib.load().pcm_cross_attn_backward_hip(*args, out32.data_ptr(), lse.data_ptr(), dout.data_ptr(), *gs, p, dq.data_ptr(),
-                                                     dk.data_ptr(), dv.data_ptr(), p + at, ws_bytes, _raw_stream())
+                                                     dk.data_ptr() if need_k or need_v else 0, dv.data_ptr() if need_k or need_v else 0, p + at,
+                                                     ws_bytes, _raw_stream())
     if rc:
         _lib.check(rc, "pcm_cross_attn_backward_hip")
-    return dq, dk, dv, None, None, None, None
+    return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
 _backward_once = once_differentiable(_backward)  # under create_graph: a second derivative is refused; otherwise its checks cost 4 us for nothing

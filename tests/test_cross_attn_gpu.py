@@ -253,3 +253,14 @@ def test_rows_shared_by_all_positions():
     q, k, v, dout = _inputs((2, 9), (2, 1), 2, 64, 4, seed=26)
     wide = lambda t: t.expand(2, 70, 2, 64)  # noqa: E731
     _check(q, wide(k), wide(v), dout, None, None, None, leaves=(q, wide(k.to(DEV)), wide(v.to(DEV)), dout))
+
+
+def test_some_gradients_only():
+    from pointcloudmatters_amd.policy import cross_attention
+
+    q, k, v, dout = _inputs((2, 40), (2, 90), 2, 64, 4, seed=27)
+    want = _run(q, k, v, dout, None, None, None)[2]
+    for keep in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        leaves = [t.to(DEV).requires_grad_(i in keep) for i, t in enumerate((q, k, v))]
+        got = torch.autograd.grad(cross_attention(*leaves), [leaves[i] for i in keep], dout.to(DEV))
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, keep)), keep
