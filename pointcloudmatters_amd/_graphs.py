@@ -9,6 +9,7 @@ stale or non-finite bias gradients after a few dozen replays (measured; tools/db
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -105,6 +106,17 @@ def captured(fn, pool=None):
 
 
 _ACCUMULATE = torch._C._functions.AccumulateGrad
+
+
+def watched(tensors):
+    """Has a call on these tensors (None among them) to go through its autograd function?  If one of them asks for a gradient, and whenever torch
+    follows the call in another way: a kernel launched past the function is invisible to it, a tangent of forward-mode differentiation
+    would be lost (the function refuses it instead), a trace would keep only the allocation of the output."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 or torch.jit.is_tracing()
 
 
 def guard_leaves(out, what):

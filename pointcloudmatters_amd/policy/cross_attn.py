@@ -148,7 +148,7 @@ def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=Non
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("cross_attention: scale must be positive and finite, got %r" % (scale,))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _graphs.watched((q, k, v)):
         out, lse = _CrossAttention.apply(q, k, v, mask, q_offset, kv_offset, scale)
         _graphs.guard_leaves(out, "cross_attention")
     else:

@@ -117,9 +117,8 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     for b, n, name in ((b_gate, f, "b_gate"), (b_up, f, "b_up"), (b_down, e, "b_down")):
         if b is not None and b.shape != (n,):
             raise ValueError("gated_ffn: %s must be (%d,), got %s" % (name, n, tuple(b.shape)))
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given)
     args = [_rows(x, e)] + [t if t is None or t.is_contiguous() else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
-    if grad:
+    if _graphs.watched(given):
         y = _graphs.guard_leaves(_GatedFFN.apply(*args, ACTIVATIONS[activation]), "gated_ffn")
     else:
         y, _ = _forward(*args, ACTIVATIONS[activation], False)

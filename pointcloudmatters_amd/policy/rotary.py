@@ -89,6 +89,6 @@ def rotary_axes(x, coords, sections, base=10000.0, interleaved=False):
         raise ValueError("rotary_axes: base must be positive, got %r" % (base,))
     if coords.stride(-1) != 1:
         coords = coords.contiguous()
-    if not (torch.is_grad_enabled() and x.requires_grad):
+    if not _graphs.watched((x,)):
         return _launch(x, coords, sections, float(base), bool(interleaved), False)
     return _graphs.guard_leaves(_RotaryAxes.apply(x, coords, sections, float(base), bool(interleaved), False), "rotary_axes")
