@@ -36,7 +36,7 @@ def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
         ld = L_.pcm_gated_ffn_hidden_ld(f)
         n = L_.pcm_gated_ffn_ws_bytes(rows, e, f, False)
         y = torch.empty((rows, e), dtype=x.dtype, device=dev)
-        size = 2 * rows * ld
+        size = 2 * int(rows) * ld  # int: while a call is traced, sizes are tensors, and addresses formed with them would be
         hidden = _empty(5 * size if keep else size + n, dev)  # without a backward pass: h, then the workspace
         p = hidden.data_ptr()
         a, u, h = (p, p + 2 * size, p + 4 * size) if keep else (0, 0, p)

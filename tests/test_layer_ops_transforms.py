@@ -56,7 +56,7 @@ def test_a_forward_mode_tangent_is_refused_not_lost(dev, op):
             assert torch.equal(f(x), f(x.clone()))  # tensors without a tangent are none of its business
 
 
-@pytest.mark.parametrize("op", [op for op in OPS if not op.startswith("gated")])
+@pytest.mark.parametrize("op", OPS)
 @pytest.mark.parametrize("grad", [False, True])
 def test_a_traced_call_computes(dev, op, grad):
     f, x = _call(op, dev)
