@@ -119,6 +119,12 @@ def watched(tensors):
     return forward_ad._current_level >= 0 or torch.jit.is_tracing()
 
 
+def refuse_tangent(dout, what):
+    """For a backward pass that runs past autograd: an incoming gradient with a forward-mode tangent is refused, not stripped of it."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(dout).tangent is not None:
+        raise NotImplementedError("%s: the backward pass has no forward-mode derivative" % what)
+
+
 def guard_leaves(out, what):
     """`out`, the result of an autograd function whose inputs may be leaves, views of them or casts -- refused during a capture when an
     eager graph over the same leaves is alive.  autograd keeps ONE accumulation node per leaf, for as long as any graph holds it, on the

@@ -74,6 +74,7 @@ class _CrossAttention(Function):
 
     @staticmethod
     def backward(ctx, dout, _):
+        _graphs.refuse_tangent(dout, "cross_attention")
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout)
 
 

@@ -59,6 +59,7 @@ class _GatedFFN(Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _graphs.refuse_tangent(dy, "gated_ffn")
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dy)
 
 

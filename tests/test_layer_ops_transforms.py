@@ -57,6 +57,19 @@ def test_a_forward_mode_tangent_is_refused_not_lost(dev, op):
 
 
 @pytest.mark.parametrize("op", OPS)
+def test_a_tangent_of_the_incoming_gradient_is_refused_not_lost(dev, op):
+    f, x = _call(op, dev)
+    leaf = x.clone().requires_grad_()
+    with forward_ad.dual_level():
+        out = f(leaf)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+    out = f(leaf)
+    (g,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert g.isfinite().all() and g.abs().sum() > 0
+
+
+@pytest.mark.parametrize("op", OPS)
 @pytest.mark.parametrize("grad", [False, True])
 def test_a_traced_call_computes(dev, op, grad):
     f, x = _call(op, dev)
