@@ -662,8 +662,8 @@ long gf_first_rows(long M, long N, long K)
     const long per = t.bm == 256 ? 1 : (t.bm == 128 ? 2 : 3), slots = 256 * per, nt = (N + t.bn - 1) / t.bn;
     const long whole = gf_tiles(M, N, t) / slots, rest = gf_tiles(M, N, t) - whole * slots;
     if (whole == 0 || rest == 0 || rest * 3 > slots || t.bm * t.bn * per * K < 1L << 24) return M;
-    const long rows = whole * slots / nt * t.bm;
-    return rows < M ? rows : M;
+    const long rows = whole * slots / nt * t.bm;  // none where one row of tiles is more than the whole rounds hold: the rows stay together
+    return rows > 0 && rows < M ? rows : M;
 }
 
 template <int EP, bool ACOL, bool BCOL>

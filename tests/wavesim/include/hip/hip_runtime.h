@@ -33,9 +33,9 @@ using wavesim::dim3;
 typedef int hipError_t;
 typedef void *hipStream_t;
 typedef void *hipDeviceptr_t;
-enum { hipSuccess = 0 };
+enum { hipSuccess = 0, hipErrorInvalidConfiguration = 9 };
 enum hipFuncAttribute { hipFuncAttributeMaxDynamicSharedMemorySize = 8 };
-inline hipError_t hipGetLastError() { return hipSuccess; }
+inline hipError_t hipGetLastError() { const int e = wavesim::g_launch_error; return wavesim::g_launch_error = 0, e; }
 template <class F> inline hipError_t hipFuncSetAttribute(F, hipFuncAttribute, int) { return hipSuccess; }
 inline hipError_t hipMemsetAsync(void *p, int v, size_t n, hipStream_t) { std::memset(p, v, n); return hipSuccess; }
 inline hipError_t hipMemsetD32Async(hipDeviceptr_t p, int v, size_t n, hipStream_t)

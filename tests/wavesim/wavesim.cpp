@@ -313,11 +313,18 @@ static void run_block(Block &b)
     }
 }
 
+int g_launch_error = 0;
+
 void launch(const std::function<void()> &body, dim3 grid, dim3 block, size_t dyn_bytes)
 {
     if (g_blk != nullptr) { std::fprintf(stderr, "wavesim: nested launch\n"); std::abort(); }
     const size_t threads = (size_t)block.x * block.y * block.z;
     if (threads == 0 || threads > 1024) { std::fprintf(stderr, "wavesim: bad block size %zu\n", threads); std::abort(); }
+    // the runtime takes no empty launch and none of 2^32 threads along an axis
+    if (!grid.x || !grid.y || !grid.z || (size_t)grid.x * block.x >> 32 || (size_t)grid.y * block.y >> 32 || (size_t)grid.z * block.z >> 32) {
+        g_launch_error = 9;
+        return;
+    }
     if (dyn_bytes > 160 * 1024) { std::fprintf(stderr, "wavesim: %zu bytes of dynamic LDS > 160 KiB\n", dyn_bytes); std::abort(); }
     if (g_dyn_smem_bytes < 160 * 1024) {
         g_dyn_smem = (char *)std::aligned_alloc(256, 160 * 1024);

@@ -109,6 +109,7 @@ template <class T> inline T from_bits(uint64_t b)
     return v;
 }
 
+extern int g_launch_error;  // what hipGetLastError reports and clears: an empty launch, or one of 2^32 threads and more, is not run
 void launch(const std::function<void()> &body, dim3 grid, dim3 block, size_t dyn_bytes);
 void note_launch(const char *kernel_expr);  // launch census: counts per call-site kernel expression
 void syncthreads();
