@@ -1072,7 +1072,6 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     if (bad) return bad;
     if (!out || (((uintptr_t)out | (uintptr_t)out32 | (uintptr_t)ws) & 15) != 0) return PCM_ERR_BAD_ARG;
     P.out = (u16 *)out, P.o32 = out32, P.lse = lse;
-    const bool few = xa_few(L, P.q_rows, q_offset != nullptr, P.G);
     P.nsplit = xa_splits(P, false);
     if (P.nsplit > 1) {
         if (!ws || ws_bytes < (long)P.nsplit * P.q_rows * H * (D + 2) * 4) return PCM_ERR_BAD_ARG;
@@ -1081,6 +1080,8 @@ extern "C" int pcm_cross_attn_forward_hip(int B, int H, int Hkv, int D, int L, l
     P.tiles = (int)xa_tiles(q_offset != nullptr, B, L, P.q_rows, P.G, XA_ROWS), P.each = q_offset ? 1 : P.tiles / B;
     const hipStream_t s = (hipStream_t)stream;
     const dim3 grid(xa_grid((long)P.tiles * Hkv * P.nsplit));
+    // xa_fill's limit on the tiles is that of workgroups of 256 threads: more than half as many stay with those
+    const bool few = xa_few(L, P.q_rows, q_offset != nullptr, P.G) && (D > 64 || grid.x < 0xFFFFF000u / 512);
     if (few && D <= 32) hipLaunchKernelGGL((pcm_xattn_few_kernel<32, 8>), grid, dim3(512), 0, s, P);
     else if (few && D <= 64) hipLaunchKernelGGL((pcm_xattn_few_kernel<64, 8>), grid, dim3(512), 0, s, P);
     else if (few) hipLaunchKernelGGL((pcm_xattn_few_kernel<128, 4>), grid, dim3(256), 0, s, P);

@@ -52,3 +52,42 @@ def test_gated_block_over_its_whole_range(host):
         if e * f > 1 << 32 or r * (e + 8) > 1 << 33 or r * (f + 64) > 1 << 36:
             continue  # refused
         assert _ffn(host, r, e, f, bias=rng.random() < 0.5)
+
+
+def _cross(host, b, h, hkv, d, l, s, q_packed=False, kv_packed=False):
+    """Forward and backward of b sequences of l rows over s keys (packed sides: l and s rows a sequence on average); () if refused."""
+    head = (b, h, hkv, d, l, b * l, P if q_packed else None, s, b * s, P if kv_packed else None)
+    rows = []
+    for n, heads in ((l, h), (s, hkv), (s, hkv)):
+        rows += [P, n * heads * d, heads * d, d]
+    ws = lambda back: host.pcm_cross_attn_ws_bytes(b, h, hkv, d, l, b * l, q_packed, s, b * s, kv_packed, back)  # noqa: E731
+    rc = host.pcm_cross_attn_forward_hip(*head, *rows, None, 0, 0.125, P, P, P, P, ws(0), None)
+    made = _good(host, (head, "forward"))
+    assert rc in (0, 2) and (rc == 0) == bool(made), (head, rc)
+    back = host.pcm_cross_attn_backward_hip(*head, *rows, None, 0, 0.125, P, P, P, l * h * d, h * d, d, P, P, P, P, P, ws(1), None)
+    assert back == rc, (head, rc, back)
+    return made + _good(host, (head, "backward"))
+
+
+@pytest.mark.parametrize("d", [8, 32, 64, 72, 128])
+def test_attention_of_single_queries_in_very_large_batches(host, d):
+    """A workgroup a (sequence, key head): up to 512 threads.  With keys the key side's limit comes first; a memory without any has none."""
+    limit = 0xFFFFF000 // 512
+    for pairs in (1 << 20, limit // 8 * 8, limit // 8 * 8 + 8, 8800000, 0xFFFFF000 // 256 // 8 * 8):
+        for hkv in (1, 8):
+            for group in (1, 4):
+                assert _cross(host, pairs // hkv, hkv * group, hkv, d, 1, 0)
+                assert bool(_cross(host, pairs // hkv, hkv * group, hkv, d, 1, 2)) == (pairs <= limit)
+    assert not _cross(host, (1 << 32) // 256, 1, 1, d, 1, 0)  # refused
+    assert any("few" in k for k, *_ in _cross(host, 1000, 8, 8, d, 1, 2))
+
+
+def test_attention_over_its_whole_range(host):
+    rng = random.Random(6)
+    log = lambda hi: int(round(2 ** rng.uniform(0, hi)))  # noqa: E731
+    for _ in range(4000):
+        hkv, group = log(5), log(5)
+        b, l, s = log(24), log(20), log(24)
+        if b * l > 1 << 31 or b * s > 1 << 31 or l * hkv * group * 128 > 1 << 40:
+            continue
+        _cross(host, b, hkv * group, hkv, 8 * rng.randint(1, 16), l, s, rng.random() < 0.5, rng.random() < 0.5)
