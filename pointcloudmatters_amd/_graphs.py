@@ -7,6 +7,7 @@ PyTorch's reductions depend on one to zero their inter-block semaphores -- a rep
 stale or non-finite bias gradients after a few dozen replays (measured; tools/dbg/graph_memset2.py, graph_reduce4.py).
 """
 import ctypes
+import weakref
 
 import torch
 from torch.autograd import forward_ad
@@ -125,27 +126,48 @@ def refuse_tangent(dout, what):
         raise NotImplementedError("%s: the backward pass has no forward-mode derivative" % what)
 
 
+_LIVE = weakref.WeakKeyDictionary()  # autograd nodes of the guarded operators' calls, while a graph holds them -> (device, stream) of the call
+
+
+def _accumulation_nodes(node):
+    found, seen, stack = set(), {node}, [node]
+    while stack:
+        for behind, _ in stack.pop().next_functions:
+            if behind is None or behind in seen:
+                continue
+            seen.add(behind)
+            if type(behind) is _ACCUMULATE:
+                found.add(behind)
+            else:
+                stack.append(behind)
+    return found
+
+
 def guard_leaves(out, what):
-    """`out`, the result of an autograd function whose inputs may be leaves, views of them or casts -- refused during a capture when an
-    eager graph over the same leaves is alive.  autograd keeps ONE accumulation node per leaf, for as long as any graph holds it, on the
-    stream it was made on; a backward pass captured on another stream then draws that stream into the capture, and ending the capture
-    ends the process (a segmentation fault inside the runtime).  Eager calls note their stream on the node; a captured call that finds
-    another one raises instead.  Freeing the eager graph (its outputs) frees the node."""
-    if out.grad_fn is None:
+    """`out`, the result of an autograd function -- refused during a capture when a graph that an earlier call of a guarded operator made on
+    another stream is alive and shares a leaf with it, however far behind either.  autograd keeps ONE accumulation node per leaf, for as
+    long as any graph holds it, on the stream it was made on; a backward pass captured on another stream then draws that stream into the
+    capture, and ending the capture ends the process (a segmentation fault inside the runtime).  Freeing the earlier graph (its outputs and
+    losses, backward done or not) frees the nodes.
+
+    What it does not see: a graph of other operations alone that holds the leaf -- autograd does not tell which stream a node is on.  What it
+    refuses for nothing: a capture that runs no backward pass; under torch.no_grad() it is not looked at."""
+    node = out.grad_fn
+    if node is None:
         return out
-    here, capturing = _lib.raw_stream(), torch.cuda.is_current_stream_capturing()
-    for node, _ in out.grad_fn.next_functions:
-        for _ in range(4):  # through what a wrapper puts in front: a view, a cast, a copy
-            if type(node) is _ACCUMULATE:
-                made = node.metadata.setdefault("pcm_stream", here)
-                if capturing and made != here:
+    with _lib.on_device(out.device):
+        here = (out.device.index, _lib.raw_stream())
+        if torch.cuda.is_current_stream_capturing():
+            mine = None
+            for ref in list(_LIVE.data):
+                other = ref()
+                if other is None or _LIVE.get(other, here) == here:
+                    continue
+                mine = _accumulation_nodes(node) if mine is None else mine
+                if not mine.isdisjoint(_accumulation_nodes(other)):
                     raise RuntimeError("%s: an eager graph over the same leaf tensors is alive: free its outputs before a backward pass "
                                        "of them is captured" % what)
-                break
-            behind = node.next_functions if node is not None else ()
-            if len(behind) != 1:
-                break
-            node = behind[0][0]
+    _LIVE[node] = here
     return out
 
 
