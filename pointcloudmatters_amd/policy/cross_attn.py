@@ -120,6 +120,7 @@ def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=Non
     key head h // (H / Hkv)); D a multiple of 8 up to 128; any strides with the channels contiguous (what 16-byte accesses do not fit is
     copied first).  key_padding_mask: bool (B, S), or (T',) for packed keys, True = ignore (the nn.MultiheadAttention convention);
     whatever stands in masked or absent rows, NaN and infinities included, has no influence.  scale: > 0, 1 / sqrt(D) by default.
+    Under bf16 autocast, q, k and v of other floating types are cast first, as linear layers do.
 
     Returns (.., H, D) like q; a row without a key is zero, so are packed rows behind the last sequence.  return_lse: also the natural
     logarithm of each row's sum of exponentials, fp32, q.shape[:-1] (-inf without a key; no gradient).  Gradients for q, k and v; results
@@ -127,8 +128,10 @@ def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=Non
     _common.require_hip(q, k, v, key_padding_mask, q_offset, kv_offset)
     if q.dim() not in (3, 4) or k.dim() not in (3, 4) or v.shape != k.shape:
         raise ValueError("cross_attention: shapes q %s, k %s, v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+        q, k, v = (t.to(torch.bfloat16) if t.is_floating_point() else t for t in (q, k, v))
     if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
-        raise TypeError("cross_attention: q, k, v must be bfloat16, got %s, %s, %s" % (q.dtype, k.dtype, v.dtype))
+        raise TypeError("cross_attention: q, k, v must be bfloat16 (or the call under bf16 autocast), got %s, %s, %s" % (q.dtype, k.dtype, v.dtype))
     if not q.device == k.device == v.device:
         raise ValueError("cross_attention: q, k, v are on %s, %s, %s" % (q.device, k.device, v.device))
     h, d = q.shape[-2:]
