@@ -430,7 +430,7 @@ __device__ __forceinline__ void xa_finish(const XaParams &P, const XaRows &R, co
         for (int i = 0; i < DP / 32; ++i) xa_store_part(P.part_o + at * P.D, P.D, h, i, o[i]);
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // l >= 1 with a key (its largest weight is 1), NaN with a NaN among the scores
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // l >= 1 with a key (the reference score's own weight is 1, the largest at most 2^8), NaN with a NaN among the scores
     if (P.lse && h == 0) P.lse[R.out_row] = l == 0.f ? -INFINITY : m * P.scale + __logf(l);
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) {
@@ -977,8 +977,9 @@ bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows
 // Splits of the keys.  A workgroup per (tile, key head) is too few for 256 compute units when the rows are few (a decoder's 100 queries): the
 // keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and re-reads its row's fp32 sums and costs a
 // second launch (4 - 7 us), so it has 256 keys at least.  The kernel of few rows shares the keys among its own waves (8, or 4 for heads wider
-// than 64) and splits only past 256 keys for each of them: one row over 2051 keys, 8 heads of 64, takes 13.4 us without a split and
-// 10.4 + 4.8 with 7.  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave hides the
+// than 64), so a split of its has 2048 keys (1024) at least, 256 a wave: one split up to 4095 keys, two up to 6143 and so on.  Measured at one
+// row over 2051 keys, 8 heads of 64: 13.4 us without a split, 10.4 + 4.8 with 7; in the kernel's time a wave's chain of tiles counts, which
+// is twice as long at 4095 keys.  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave hides the
 // others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 230 us with one split, 173 + 7
 // for the joining with two, 167 + 10 with four).
 int xa_splits(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, bool backward)
