@@ -978,10 +978,10 @@ bool xa_few(int L, long q_rows, int q_packed, int G) { return (q_packed ? q_rows
 // keys are then shared out until about 512 workgroups run, two a compute unit.  A split writes and re-reads its row's fp32 sums and costs a
 // second launch (4 - 7 us), so it has 256 keys at least.  The kernel of few rows shares the keys among its own waves (8, or 4 for heads wider
 // than 64), so a split of its has 2048 keys (1024) at least, 256 a wave: one split up to 4095 keys, two up to 6143 and so on.  Measured at one
-// row over 2051 keys, 8 heads of 64: 13.4 us without a split, 10.4 + 4.8 with 7; in the kernel's time a wave's chain of tiles counts, which
-// is twice as long at 4095 keys.  Long states are shared out further, to three workgroups a compute unit and two rounds of them: a third wave hides the
-// others' waits, and ragged sequences even out (4500 rows over 12000 keys on average, 8 heads of 64: 230 us with one split, 173 + 7
-// for the joining with two, 167 + 10 with four).
+// row over 2051 keys, 8 heads of 64: 13.4 us without a split, 10.4 + 4.8 with 7.  What counts is a wave's chain of tiles, so a call takes 16.2 us
+// over 2051 keys, 19.6 over 4095 and, with two splits, 16.2 over 4096 and 20.6 over 6143.  Long states are shared out further, to three
+// workgroups a compute unit and two rounds of them: a third wave hides the others' waits, and ragged sequences even out (4500 rows over 12000
+// keys on average, 8 heads of 64: 230 us with one split, 173 + 7 for the joining with two, 167 + 10 with four).
 int xa_splits(int B, int H, int Hkv, int D, int L, long q_rows, int q_packed, int S, long kv_rows, int kv_packed, bool backward)
 {
     const int G = H / Hkv;
