@@ -117,16 +117,20 @@ def watched(tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return forward_ad._current_level >= 0 or torch.jit.is_tracing()
+    return forward_ad._current_level >= 0 or torch._C._is_tracing()
+
+
+def has_tangent(t):
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def refuse_tangent(dout, what):
     """For a backward pass that runs past autograd: an incoming gradient with a forward-mode tangent is refused, not stripped of it."""
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(dout).tangent is not None:
+    if has_tangent(dout):
         raise NotImplementedError("%s: the backward pass has no forward-mode derivative" % what)
 
 
-_LIVE = weakref.WeakKeyDictionary()  # autograd nodes of the guarded operators' calls, while a graph holds them -> (device, stream) of the call
+_LIVE = {}  # weak reference to the autograd node of a guarded operator's call, while a graph holds it -> (device, stream) of the call
 
 
 def _accumulation_nodes(node):
@@ -159,15 +163,15 @@ def guard_leaves(out, what):
         here = (out.device.index, _lib.raw_stream())
         if torch.cuda.is_current_stream_capturing():
             mine = None
-            for ref in list(_LIVE.data):
+            for ref in list(_LIVE):
                 other = ref()
-                if other is None or _LIVE.get(other, here) == here:
+                if other is None or _LIVE.get(ref) in (None, here):
                     continue
                 mine = _accumulation_nodes(node) if mine is None else mine
                 if not mine.isdisjoint(_accumulation_nodes(other)):
                     raise RuntimeError("%s: an eager graph over the same leaf tensors is alive: free its outputs before a backward pass "
                                        "of them is captured" % what)
-    _LIVE[node] = here
+    _LIVE[weakref.ref(node, _LIVE.pop)] = here
     return out
 
 

@@ -128,10 +128,11 @@ def cross_attention(q, k, v, key_padding_mask=None, q_offset=None, kv_offset=Non
     _common.require_hip(q, k, v, key_padding_mask, q_offset, kv_offset)
     if q.dim() not in (3, 4) or k.dim() not in (3, 4) or v.shape != k.shape:
         raise ValueError("cross_attention: shapes q %s, k %s, v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
-        q, k, v = (t.to(torch.bfloat16) if t.is_floating_point() else t for t in (q, k, v))
     if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
-        raise TypeError("cross_attention: q, k, v must be bfloat16 (or the call under bf16 autocast), got %s, %s, %s" % (q.dtype, k.dtype, v.dtype))
+        if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+            q, k, v = (t.to(torch.bfloat16) if t.is_floating_point() else t for t in (q, k, v))
+        if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+            raise TypeError("cross_attention: q, k, v must be bfloat16 (or the call under bf16 autocast), got %s, %s, %s" % (q.dtype, k.dtype, v.dtype))
     if not q.device == k.device == v.device:
         raise ValueError("cross_attention: q, k, v are on %s, %s, %s" % (q.device, k.device, v.device))
     h, d = q.shape[-2:]

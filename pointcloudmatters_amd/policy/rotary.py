@@ -55,7 +55,7 @@ class _RotaryAxes(Function):
     @staticmethod
     def backward(ctx, dout):
         (coords,) = ctx.saved_tensors
-        turn = _RotaryAxes.apply if _graphs.watched((dout,)) else _launch  # linear: its own backward, turned back
+        turn = _RotaryAxes.apply if dout.requires_grad and torch.is_grad_enabled() or _graphs.has_tangent(dout) else _launch  # linear: its own backward, turned back
         return turn(dout, coords, *ctx.meta), None, None, None, None, None
 
 
